@@ -164,6 +164,92 @@ int rnet_cross_entropy_forward_noalloc(const float* logits, const int* targets, 
 int rnet_residual_add(float* x, const float* y, size_t n, void* stream);
 int rnet_scale_grads(float* grads, float scale, size_t n, void* stream);
 
+/* ------------------------------------------------------------------ logits
+ * Operators on the logits of a model (no counterpart in the reference). Rows
+ * of logits are fp32 or bf16 with a pitch of `ld` elements (ld >= vocab, any
+ * alignment of the element size). All arithmetic is fp32 or wider. */
+#define RNET_DTYPE_F32 0
+#define RNET_DTYPE_BF16 1
+
+/* The record a teacher keeps of each row: its top_k (1..64, <= vocab) largest
+ * logits, sorted, ties to the lowest index. top_logits / top_idx are [rows,
+ * top_k]; lse (may be NULL) is [rows]: log sum exp(logit / temperature) over
+ * the whole row. A NaN logit counts as -inf, +inf as the largest finite fp32.
+ * Places beyond the row's logits above -inf hold -inf / -1 (padding that the
+ * distillation skips). */
+int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float temperature,
+                             float* top_logits, int* top_idx, float* lse, int rows, int vocab,
+                             int top_k, void* stream);
+
+/* Distillation from such records, loss and gradient in one call, like
+ * rnet_cross_entropy_forward. With z a row's logits, q = softmax(z /
+ * temperature), p_k the teacher's probabilities and w = row_weight[row]:
+ *   row_loss = w * (soft_weight * temperature^2 * sum_k p_k (log p_k - log q[i_k])
+ *                   + hard_weight * (log sum exp(z) - z[target]))
+ *   dlogits  = grad_scale * d row_loss / d z
+ *   loss     = sum of row_loss (one float; a fixed order, may be NULL)
+ * teacher_idx / teacher_logits [rows, top_k]: an index < 0 is padding, the same
+ * index may come twice. teacher_lse NULL: p = softmax(teacher_logits /
+ * temperature) over the row's entries (a row without entries has no soft
+ * part); else p_k = exp(teacher_logits / temperature - teacher_lse), as
+ * recorded at the same temperature, and the mass outside the record is left
+ * out of the sum. targets [rows] (needed when hard_weight != 0): a negative
+ * target has no hard part. row_weight [rows] (NULL = 1): a row of weight 0
+ * gives exactly 0 loss and gradient whatever its logits and record hold. A row
+ * whose logits are all -inf has no distribution and gives 0; a NaN or +inf
+ * logit makes its row NaN. A teacher index or target >= vocab is skipped and
+ * sets the device error word (bit 1). dlogits (may be NULL: loss only) has the
+ * logits' type and a pitch of ld_dlogits; it may be the logits themselves
+ * (same pointer and pitch). vocab <= 262144, top_k 1..64. */
+int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const int* teacher_idx,
+                              const float* teacher_logits, const float* teacher_lse,
+                              const int* targets, const float* row_weight, float temperature,
+                              float soft_weight, float hard_weight, float grad_scale,
+                              float* row_loss, float* loss, void* dlogits, long long ld_dlogits,
+                              int rows, int vocab, int top_k, void* stream);
+
+/* ------------------------------------------------------------------ beam search
+ * Streams are [batch * beams]: the beams of a sequence lie together, beams
+ * 1..32. (No counterpart in the reference.)
+ *
+ * One selection: per sequence, the `beams` candidates (b, v) with the largest
+ * scores_in[b] + log softmax(logits[b])[v], sorted, ties to the lowest
+ * b * vocab + v. Totals are compared in 64 bits. finished_in[b] != 0 (NULL =
+ * none finished; needs eos >= 0): the beam has ended and offers only
+ * (b, eos) at its own score. Outputs [batch * beams]: scores, tokens, parents
+ * (the beam 0..beams-1 each one continues) and finished (may be NULL without
+ * finished_in) = the parent had finished, or token == eos (eos = -1: no token
+ * ends a beam). A NaN logit or score counts as -inf, +inf as the largest
+ * finite fp32; candidates at -inf are never taken. A sequence with fewer
+ * candidates than beams fills the places left with score -inf, parent = the
+ * place itself and token = eos (0 without one). So a search starts with scores
+ * {0, -inf, ...}. scores / finished may be scores_in / finished_in. */
+int rnet_beam_select(const void* logits, int dtype, long long ld, const float* scores_in,
+                     const int* finished_in, int eos, float* scores, int* tokens, int* parents,
+                     int* finished, int batch, int beams, int vocab, void* stream);
+
+/* States follow their beams: in each of `outer` planes (outer_pitch bytes
+ * apart) of batch * beams rows (row_pitch bytes apart, row_bytes long), row j of
+ * a sequence becomes its old row parents[j]. dst may be src (in place: rows
+ * that stay are not touched); otherwise the two must not overlap, and share
+ * the pitches. Rows, pitches and pointers are multiples of 4 bytes. A parent
+ * outside 0..beams-1 leaves its row as it is and sets the device error word
+ * (bit 1). Bytes between the rows are not touched. */
+int rnet_beam_reorder(const void* src, void* dst, size_t row_bytes, size_t row_pitch, size_t outer,
+                      size_t outer_pitch, const int* parents, int batch, int beams, void* stream);
+
+/* The sequences behind the last beams. tokens / parents [n_steps, batch *
+ * beams] are the recorded outputs of n_steps >= 1 selections, scores [batch *
+ * beams] the last one's. sequences [batch * beams, n_steps]: per sequence the
+ * beams sorted by score / length^length_alpha (64 bits, ties to the lower
+ * beam); length counts the tokens up to and including the first eos (n_steps
+ * without one, or with eos < 0), and eos fills what follows. lengths and
+ * ranked_scores [batch * beams] are in the same order. A parent outside
+ * 0..beams-1 counts as the beam itself and sets the device error word (bit 1). */
+int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
+                        float length_alpha, int* sequences, int* lengths, float* ranked_scores,
+                        int n_steps, int batch, int beams, void* stream);
+
 /* ------------------------------------------------------------------ data
  * Training batches of the reference's DataLoader (src/data_loader.cpp:31-52
  * as driven by src/main.cpp:117-133) with the corpus resident on the GPU.

@@ -20,6 +20,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
 
 
 class RnetError(RuntimeError):
@@ -40,6 +41,9 @@ class ModelConfig(ctypes.Structure):
              seq_len=256, eps=1e-6, n_heads=8):
         return cls(d_model, n_layers, d_ff, n_heads, d_model, n_slots, top_k, vocab, seq_len, eps)
 
+
+# element types of the operators on logits
+DTYPE_F32, DTYPE_BF16 = 0, 1
 
 # name -> argtypes (all return int status)
 _SIGS = {
@@ -65,6 +69,12 @@ _SIGS = {
     "rnet_swiglu_backward": [_P] * 11 + [_I, _I, _I, _P],
     "rnet_cross_entropy_forward": [_P, _P, _P, _P, _I, _I, _P],
     "rnet_cross_entropy_forward_noalloc": [_P, _P, _P, _P, _I, _I, _P],
+    "rnet_topk_logits_forward": [_P, _I, _LL, _F, _P, _P, _P, _I, _I, _I, _P],
+    "rnet_distill_topk_forward": [_P, _I, _LL] + [_P] * 5 + [_F] * 4 + [_P] * 3 +
+                                 [_LL, _I, _I, _I, _P],
+    "rnet_beam_select": [_P, _I, _LL, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P],
+    "rnet_beam_reorder": [_P, _P, _SZ, _SZ, _SZ, _SZ, _P, _I, _I, _P],
+    "rnet_beam_backtrack": [_P, _P, _P, _I, _F, _P, _P, _P, _I, _I, _I, _P],
     "rnet_residual_add": [_P, _P, _SZ, _P],
     "rnet_scale_grads": [_P, _F, _SZ, _P],
     "rnet_model_create": [ctypes.POINTER(ModelConfig), _I, _I, ctypes.POINTER(_P)],

@@ -4,6 +4,11 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+// Limits of the operators on logits and beams (also in the messages of the C ABI).
+#define RNET_TOPK_MAX 64
+#define RNET_BEAMS_MAX 32
+#define RNET_DISTILL_VOCAB_MAX 262144
+
 namespace rnet_k {
 
 // Launch bookkeeping: count `n` kernels launched by this library and return
@@ -150,6 +155,42 @@ cudaError_t argmax_rows(const float* logits, int M, int V, int* tok, int* out, i
 // sampled token = *pos + advance); advance = 1 advances *pos afterwards.
 cudaError_t sample_rows(const float* logits, int M, int V, float temperature, float top_p,
                         unsigned long long seed, int* tok, int* pos, int advance, cudaStream_t s);
+
+// ---- top-logit records and distillation (logits_ops.cu) --------------------
+// Logits are fp32 or bf16 rows with a pitch of ld elements.
+// top / idx [rows, K]: the K largest logits of each row, ties to the lowest
+// index (NaN counts as -inf, +inf as the largest finite number); places beyond
+// the row's logits above -inf get -inf / -1. lse (optional) [rows]:
+// log sum exp(logit / tau).
+cudaError_t topk_logits(const void* logits, bool bf16, long long ld, float tau, float* top,
+                        int* idx, float* lse, int rows, int V, int K, cudaStream_t s);
+// Loss of each row against a teacher's record, and the gradient:
+//   row_loss = w (soft tau^2 sum_k p_k (log p_k - log softmax(z/tau)[i_k]) + hard CE(z, target))
+//   dl = scale * d row_loss / dz            (dl may be null, or the logits themselves)
+// p = softmax(t_val / tau) over the entries with i_k >= 0, or
+// exp(t_val / tau - t_lse) if t_lse is given. loss (optional) = sum row_loss.
+cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int* t_idx,
+                         const float* t_val, const float* t_lse, const int* targets,
+                         const float* weight, float tau, float soft, float hard, float scale,
+                         float* row_loss, float* loss, void* dlogits, long long ldd, int rows,
+                         int V, int K, unsigned* err, cudaStream_t s);
+
+// ---- beam search (beam.cu) --------------------------------------------------
+// Per sequence, the `beams` best of score[b] + log softmax(logits[b])[v] over
+// (b, v), ties to the lowest b * V + v; a finished beam offers (b, eos) at its
+// own score only. Outputs may be the inputs of the same name.
+cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float* scores_in,
+                        const int* finished_in, int eos, float* scores, int* tokens, int* parents,
+                        int* finished, int batch, int beams, int V, cudaStream_t s);
+// dst row j of each group of `beams` rows = src row parents[j]; dst may be src.
+cudaError_t beam_reorder(const void* src, void* dst, size_t row_bytes, size_t pitch, size_t outer,
+                         size_t outer_pitch, const int* parents, int batch, int beams,
+                         unsigned* err, cudaStream_t s);
+// Follows the recorded parents [steps, batch * beams] back from the last step;
+// sequences [batch * beams, steps] ranked by score / length^alpha.
+cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
+                           float alpha, int* sequences, int* lengths, float* ranked, int steps,
+                           int batch, int beams, unsigned* err, cudaStream_t s);
 
 // ---- optimizer (optimizer.cu) ---------------------------------------------
 // Global-norm clip + SGD over one flat buffer, no host synchronisation:

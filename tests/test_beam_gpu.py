@@ -1,0 +1,302 @@
+"""Beam selection, state reordering and backtracking on the GPU, against the
+plain 64-bit forms of logits_oracle.py. Tokens, parents and order are compared
+exactly: every input's candidates are further apart than GAP, which is more
+than the kernels' log-normalisers may be off."""
+import numpy as np
+import pytest
+
+import logits_oracle as ref
+
+pytestmark = pytest.mark.gpu
+
+GAP = 1e-6
+
+
+def _t(torch, a, ty=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if ty is None else t.to(ty)
+
+
+def _logits(torch, z, dtype, pad=0, offset=0):
+    t = torch.float32 if dtype == "f32" else torch.bfloat16
+    n, v = z.shape
+    buf = torch.full((n * (v + pad) + offset + 8,), 7.0, dtype=t, device="cuda")
+    view = buf[offset:offset + n * (v + pad)].view(n, v + pad)[:, :v]
+    view.copy_(_t(torch, z).to(t))
+    return view
+
+
+def _select(rnet, torch, z, dtype, scores, beams, eos=-1, finished=None, stream=None):
+    m, v = z.shape
+    s = _t(torch, np.asarray(scores, np.float32))
+    f = None if finished is None else _t(torch, np.asarray(finished, np.int32))
+    out = torch.full((m,), 3.0, device="cuda")
+    ints = [torch.full((m,), 55, dtype=torch.int32, device="cuda") for _ in range(3)]
+    rnet.call("rnet_beam_select", z.data_ptr(), int(dtype == "bf16"), z.stride(0), s.data_ptr(),
+              None if f is None else f.data_ptr(), eos, out.data_ptr(), ints[0].data_ptr(),
+              ints[1].data_ptr(), ints[2].data_ptr(), m // beams, beams, v, stream)
+    torch.cuda.synchronize()
+    return out.cpu().numpy(), *[i.cpu().numpy() for i in ints]
+
+
+def _check_select(rnet, torch, z, dtype, scores, beams, eos=-1, finished=None, gap=GAP):
+    zz = z.detach().float().cpu().numpy()
+    want = ref.select(zz, scores, beams, eos, finished)
+    assert want[4] > gap, "the input's candidates lie too close together"
+    got = _select(rnet, torch, z, dtype, scores, beams, eos, finished)
+    for name, a, b in zip(("tokens", "parents", "finished"), got[1:], want[1:4]):
+        np.testing.assert_array_equal(a, b, err_msg=name)
+    fin = np.isfinite(want[0])
+    np.testing.assert_array_equal(got[0][~fin], want[0][~fin].astype(np.float32))
+    bound = ref.lse_bound(want[0], z.shape[1]) + np.abs(np.where(fin, want[0], 0)) * ref.U
+    assert np.all(np.abs(got[0] - want[0])[fin] <= bound[fin])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("batch,beams,v,pad,offset", [
+    (1, 1, 1, 0, 0), (1, 4, 256, 0, 0), (32, 8, 256, 0, 0), (3, 5, 7, 2, 1), (2, 32, 2, 0, 0),
+    (2, 32, 33, 0, 0), (2, 32, 1024, 0, 0), (3, 3, 1025, 0, 1), (5, 8, 1000, 1, 0),
+    (1, 8, 4099, 0, 0), (2, 4, 50001, 0, 0), (1, 32, 20000, 3, 0), (1, 2, 262145, 0, 1),
+    (70, 4, 3001, 0, 0), (400, 2, 100, 0, 0)])
+def test_select(rnet, cuda, dtype, batch, beams, v, pad, offset):
+    r = np.random.default_rng(batch * 1000 + beams * 10 + v)
+    m = batch * beams
+    z = _logits(cuda, (r.normal(size=(m, v)) * 2.5).astype(np.float32), dtype, pad, offset)
+    scores = (-4 * r.random(m)).astype(np.float32)
+    _check_select(rnet, cuda, z, dtype, scores, beams)
+    fin = (r.random(m) < 0.3).astype(np.int32)
+    _check_select(rnet, cuda, z, dtype, scores, beams, eos=v - 1, finished=fin)
+
+
+@pytest.mark.parametrize("v", [5, 255, 1023, 2047, 30001])
+def test_select_ties_go_to_the_lowest_candidate(rnet, cuda, v):
+    """Equal rows give equal log-normalisers, so their candidates tie exactly."""
+    torch, beams = cuda, 6
+    r = np.random.default_rng(v)
+    row = (r.normal(size=(1, v)) * 2).astype(np.float32)
+    z = _logits(torch, np.repeat(row, 2 * beams, 0), "f32", 0, 1)
+    _check_select(rnet, torch, z, "f32", np.full(2 * beams, -1.5, np.float32), beams)
+    z = _logits(torch, np.round(np.repeat(row, 2 * beams, 0)), "f32", 3)
+    _check_select(rnet, torch, z, "f32", np.full(2 * beams, -1.5, np.float32), beams, eos=0)
+    _check_select(rnet, torch, _logits(torch, np.zeros((beams, v), np.float32), "bf16"), "bf16",
+                  np.zeros(beams, np.float32), beams)
+
+
+@pytest.mark.parametrize("v", [40, 700, 9000])
+def test_select_first_step_and_masked_rows(rnet, cuda, v):
+    torch, beams = cuda, 4
+    r = np.random.default_rng(v)
+    z = (r.normal(size=(5 * beams, v)) * 2).astype(np.float32)
+    scores = (-r.random(5 * beams)).astype(np.float32)
+    scores[:beams] = [0, -np.inf, -np.inf, -np.inf]      # a search begins
+    z[beams:2 * beams] = -np.inf                          # nothing is allowed at all
+    z[2 * beams:3 * beams, 3:] = -np.inf                  # fewer candidates than beams in a row
+    z[3 * beams:3 * beams + 3] = -np.inf
+    z[3 * beams + 3, 2:] = -np.inf                        # two candidates for four beams
+    z[4 * beams, 5], z[4 * beams + 1, ::2] = np.inf, np.nan
+    scores[4 * beams + 2] = np.nan
+    for fin in (None, np.eye(1, 5 * beams, 3 * beams + 1, dtype=np.int32)[0]):
+        _check_select(rnet, torch, _logits(torch, z, "f32"), "f32", scores, beams,
+                      eos=-1 if fin is None else 1, finished=fin)
+
+
+@pytest.mark.parametrize("v", [256, 20000])
+def test_select_finished_beams(rnet, cuda, v):
+    torch, beams = cuda, 8
+    r = np.random.default_rng(1)
+    m = 3 * beams
+    z = (r.normal(size=(m, v)) * 2).astype(np.float32)
+    scores = (-2 * r.random(m)).astype(np.float32)
+    fin = np.zeros(m, np.int32)
+    fin[:beams] = 1                # a sequence that has ended
+    fin[beams + 2] = 7
+    z[beams + 2] = np.nan          # its row may hold anything
+    z[2 * beams:, 4] += 30.0       # every beam ends now
+    _check_select(rnet, torch, _logits(torch, z, "f32"), "f32", scores, beams, 4, fin)
+
+
+def test_select_in_place_on_scores(rnet, cuda):
+    torch, beams, v, m = cuda, 4, 300, 12
+    for v in (300, 12000):
+        r = np.random.default_rng(v)
+        z = _logits(torch, r.normal(size=(m, v)).astype(np.float32), "f32")
+        scores, fin = (-r.random(m)).astype(np.float32), (r.random(m) < 0.4).astype(np.int32)
+        want = _select(rnet, torch, z, "f32", scores, beams, 0, fin)
+        s, f = _t(torch, scores), _t(torch, fin)
+        tok, par = (torch.empty(m, dtype=torch.int32, device="cuda") for _ in range(2))
+        rnet.call("rnet_beam_select", z.data_ptr(), 0, v, s.data_ptr(), f.data_ptr(), 0,
+                  s.data_ptr(), tok.data_ptr(), par.data_ptr(), f.data_ptr(), m // beams, beams, v,
+                  None)
+        torch.cuda.synchronize()
+        for a, b in zip((s, tok, par, f), want):
+            np.testing.assert_array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("outer,batch,beams,row,pad", [
+    (1, 1, 1, 4, 0), (1, 1, 4, 960, 0), (8, 3, 8, 7680, 0), (2, 5, 3, 7, 0), (3, 2, 32, 50, 6),
+    (2, 2, 17, 1028, 4), (1, 300, 2, 36, 0), (5, 1, 16, 33, 1)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_reorder(rnet, cuda, outer, batch, beams, row, pad, in_place):
+    torch = cuda
+    r = np.random.default_rng(outer + row)
+    m, pitch = batch * beams, row + pad
+    plane = m * pitch + (4 if pad % 4 == 0 else 3)
+    x = r.integers(0, 1 << 30, size=outer * plane).astype(np.int32)
+    par = r.integers(0, beams, size=m).astype(np.int32)
+    src, dst = _t(torch, x), torch.full((outer * plane,), 5, dtype=torch.int32, device="cuda")
+    P = _t(torch, par)
+    out = src if in_place else dst
+    rnet.call("rnet_beam_reorder", src.data_ptr(), out.data_ptr(), row * 4, pitch * 4, outer,
+              plane * 4, P.data_ptr(), batch, beams, None)
+    torch.cuda.synchronize()
+    want = x.copy() if in_place else np.full_like(x, 5)
+    for o in range(outer):
+        old = x[o * plane:o * plane + m * pitch].reshape(batch, beams, pitch)
+        new = want[o * plane:o * plane + m * pitch].reshape(batch, beams, pitch)
+        for g in range(batch):
+            new[g, :, :row] = old[g, par[g * beams:(g + 1) * beams], :row]
+    np.testing.assert_array_equal(out.cpu().numpy(), want)
+    if not in_place:
+        np.testing.assert_array_equal(src.cpu().numpy(), x)
+
+
+def test_reorder_bad_parents_stay(rnet, cuda):
+    torch = cuda
+    rnet.device_error(clear=True)
+    x = np.arange(4 * 8, dtype=np.int32)
+    s, par = _t(torch, x), _t(torch, np.array([1, -1, 4, 0], np.int32))
+    rnet.call("rnet_beam_reorder", s.data_ptr(), s.data_ptr(), 32, 32, 1, 0, par.data_ptr(), 1, 4,
+              None)
+    assert rnet.device_error(clear=True) == 2
+    want = x.reshape(4, 8)[[1, 1, 2, 0]]
+    np.testing.assert_array_equal(s.cpu().numpy().reshape(4, 8), want)
+
+
+def test_reorder_past_32_bits(rnet, cuda):
+    """Rows and planes whose byte offsets pass 2^32."""
+    torch = cuda
+    pitch, outer_pitch = (1 << 31) + 64, 3 * ((1 << 31) + 64) + 64
+    buf = torch.zeros((outer_pitch + 2 * pitch + 64) // 4, dtype=torch.int32, device="cuda")
+    rows = torch.as_strided(buf, (2, 3, 16), (outer_pitch // 4, pitch // 4, 1))
+    x = np.arange(96, dtype=np.int32).reshape(2, 3, 16)
+    rows.copy_(_t(torch, x))
+    par = _t(torch, np.array([2, 0, 1], np.int32))
+    rnet.call("rnet_beam_reorder", buf.data_ptr(), buf.data_ptr(), 64, pitch, 2, outer_pitch,
+              par.data_ptr(), 1, 3, None)
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(rows.cpu().numpy(), x[:, [2, 0, 1]])
+
+
+def _backtrack(rnet, torch, tok, par, scores, beams, eos, alpha):
+    t, m = tok.shape
+    seq = torch.full((m, t), 99, dtype=torch.int32, device="cuda")
+    ln = torch.full((m,), 99, dtype=torch.int32, device="cuda")
+    rk = torch.full((m,), 99.0, device="cuda")
+    T, P, S = _t(torch, tok), _t(torch, par), _t(torch, scores)
+    rnet.call("rnet_beam_backtrack", T.data_ptr(), P.data_ptr(), S.data_ptr(), eos, alpha,
+              seq.data_ptr(), ln.data_ptr(), rk.data_ptr(), t, m // beams, beams, None)
+    torch.cuda.synchronize()
+    return seq.cpu().numpy(), ln.cpu().numpy(), rk.cpu().numpy()
+
+
+@pytest.mark.parametrize("t,batch,beams", [(1, 1, 1), (1, 3, 5), (2, 2, 32), (31, 2, 4),
+                                           (32, 1, 7), (33, 40, 3), (257, 5, 8), (1000, 1, 32),
+                                           (4097, 2, 4)])
+@pytest.mark.parametrize("eos,alpha", [(-1, 0.0), (3, 0.0), (3, 0.7)])
+def test_backtrack(rnet, cuda, t, batch, beams, eos, alpha):
+    r = np.random.default_rng(t + beams)
+    m = batch * beams
+    tok = r.integers(0, max(6, 2 * t), size=(t, m)).astype(np.int32)
+    par = r.integers(0, beams, size=(t, m)).astype(np.int32)
+    scores = (-10 * r.random(m)).astype(np.float32)
+    if m > 2:
+        scores[1] = scores[0]
+        scores[m - 1] = -np.inf
+    seq, ln, rk = _backtrack(rnet, cuda, tok, par, scores, beams, eos, alpha)
+    s0, l0, r0 = ref.backtrack(tok, par, scores, beams, eos, alpha)
+    np.testing.assert_array_equal(ln, l0)
+    np.testing.assert_array_equal(seq, s0)
+    fin = np.isfinite(r0)
+    np.testing.assert_array_equal(rk[~fin], r0[~fin])
+    assert np.all(np.abs(rk - r0)[fin] <= 2 * ref.U * np.abs(r0[fin]))
+
+
+def test_backtrack_bad_parents(rnet, cuda):
+    rnet.device_error(clear=True)
+    tok = np.arange(12, dtype=np.int32).reshape(4, 3)
+    par = np.array([[0, 0, 0], [0, 5, 1], [2, 1, -1], [1, 2, 0]], np.int32)
+    seq, _, _ = _backtrack(rnet, cuda, tok, par, np.array([-1, -2, -3], np.float32), 3, -1, 0.0)
+    assert rnet.device_error(clear=True) == 2
+    np.testing.assert_array_equal(seq, ref.backtrack(tok, par, np.array([-1., -2, -3]), 3, -1,
+                                                     0.0)[0])
+
+
+def test_a_search_over_a_table_of_transitions(rnet, cuda):
+    """Select, reorder and backtrack together, captured as one step and
+    replayed: logits depend on the last two tokens, the state holds the older
+    one. The oracle keeps whole sequences instead."""
+    torch = cuda
+    batch, beams, v, steps, eos, alpha = 3, 5, 50, 12, 0, 0.8
+    m = batch * beams
+    r = np.random.default_rng(11)
+    table = (r.normal(size=(v, v, v)) * 1.5).astype(np.float32)
+    T = _t(torch, table)
+    state = torch.zeros(m, 4, dtype=torch.int32, device="cuda")  # last token in column 0
+    prev = torch.zeros(m, dtype=torch.int64, device="cuda")
+    first = r.integers(1, v, size=batch)
+    tok = _t(torch, np.repeat(first, beams).astype(np.int32))
+    scores = _t(torch, np.tile(np.array([0] + [-np.inf] * (beams - 1), np.float32), batch))
+    fin = torch.zeros(m, dtype=torch.int32, device="cuda")
+    par = torch.zeros(m, dtype=torch.int32, device="cuda")
+    logits = torch.zeros(m, v, device="cuda")
+    hist = torch.zeros(2, steps, m, dtype=torch.int32, device="cuda")
+
+    def step(stream):
+        logits.copy_(T[state[:, 0].long(), tok.long()])
+        state[:, 0] = tok
+        rnet.call("rnet_beam_select", logits.data_ptr(), 0, v, scores.data_ptr(), fin.data_ptr(),
+                  eos, scores.data_ptr(), tok.data_ptr(), par.data_ptr(), fin.data_ptr(), batch,
+                  beams, v, stream.cuda_stream)
+        rnet.call("rnet_beam_reorder", state.data_ptr(), state.data_ptr(), 16, 16, 1, 0,
+                  par.data_ptr(), batch, beams, stream.cuda_stream)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(side)
+        hist[0, 0].copy_(tok)
+        hist[1, 0].copy_(par)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(side)
+    for i in range(1, steps):
+        g.replay()
+        hist[0, i].copy_(tok)
+        hist[1, i].copy_(par)
+    torch.cuda.synchronize()
+    seq, ln, rk = _backtrack(rnet, torch, hist[0].cpu().numpy(), hist[1].cpu().numpy(),
+                             scores.cpu().numpy(), beams, eos, alpha)
+    # oracle: lists of (score, tokens, ended)
+    logp = table.astype(np.float64) - ref.logsumexp(table.astype(np.float64))[..., None]
+    for b in range(batch):
+        live = [(0.0, [0, int(first[b])], False)]
+        for _ in range(steps):
+            new = []
+            for i, (s, t, done) in enumerate(live):
+                if done:
+                    new.append((s, i, eos, t, True))
+                else:
+                    new += [(s + logp[t[-2], t[-1], w], i, w, t, w == eos) for w in range(v)]
+            new.sort(key=lambda c: (-c[0], c[1], c[2]))
+            live = [(s, t + [w], done) for s, _, w, t, done in new[:beams]]
+        rows = []
+        for s, t, _ in live:
+            t = t[2:]
+            n = t.index(eos) + 1 if eos in t else steps
+            rows.append((s / n ** alpha, t, n))
+        rows.sort(key=lambda c: -c[0])
+        for j, (s, t, n) in enumerate(rows):
+            assert list(seq[b * beams + j]) == t and ln[b * beams + j] == n
+            # fp32 scores round once a step; the kernels' normalisers add their own error
+            assert abs(rk[b * beams + j] - s) <= steps * (abs(s) * n ** alpha + 60) * ref.U
