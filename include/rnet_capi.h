@@ -167,7 +167,8 @@ int rnet_scale_grads(float* grads, float scale, size_t n, void* stream);
 /* ------------------------------------------------------------------ logits
  * Operators on the logits of a model (no counterpart in the reference). Rows
  * of logits are fp32 or bf16 with a pitch of `ld` elements (ld >= vocab, any
- * alignment of the element size). All arithmetic is fp32 or wider. */
+ * alignment of the element size). All arithmetic is fp32 or wider. A
+ * temperature lies within 1e-4 and 1e4. */
 #define RNET_DTYPE_F32 0
 #define RNET_DTYPE_BF16 1
 

@@ -49,8 +49,8 @@ int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float 
   NEED(ld >= vocab, "topk_logits_forward: row pitch below vocab");
   NEED(top_k >= 1 && top_k <= RNET_TOPK_MAX && top_k <= vocab,
        "topk_logits_forward: " + TOPK_RANGE + " and not above vocab");
-  NEED(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(1.0f / temperature),
-       "topk_logits_forward: temperature must be positive and finite");
+  NEED(temperature >= 1e-4f && temperature <= 1e4f,
+       "topk_logits_forward: temperature must be within 1e-4 and 1e4");
   NEED(aligned(logits, elem(dtype)) && aligned(top_logits, 4) && aligned(top_idx, 4) &&
            aligned(lse, 4),
        "topk_logits_forward: a pointer is not aligned to its element size");
@@ -76,8 +76,8 @@ int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const
                              "distill_topk_forward: vocab above " +
                                  std::to_string(RNET_DISTILL_VOCAB_MAX));
   NEED(top_k >= 1 && top_k <= RNET_TOPK_MAX, "distill_topk_forward: " + TOPK_RANGE);
-  NEED(std::isfinite(temperature) && temperature > 0.0f && std::isfinite(1.0f / temperature),
-       "distill_topk_forward: temperature must be positive and finite");
+  NEED(temperature >= 1e-4f && temperature <= 1e4f,
+       "distill_topk_forward: temperature must be within 1e-4 and 1e4");
   NEED(std::isfinite(soft_weight) && std::isfinite(hard_weight) && std::isfinite(grad_scale),
        "distill_topk_forward: weights and grad_scale must be finite");
   NEED(hard_weight == 0.0f || targets, "distill_topk_forward: hard_weight needs targets");

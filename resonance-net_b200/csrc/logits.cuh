@@ -47,10 +47,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
+// log2 x, absolute error below 2^-22 near 1, relative 2^-22 elsewhere.
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The largest value of a warp; NaN loses against any number.
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -58,42 +66,40 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// log2 of a softmax term: (x - m) c, c = log2(e) / tau, with the product and
+// the difference in one rounding: the shift is the rounded m c, the same in
+// every term and in the sum, so its rounding cancels. Where m c could leave
+// fp32 (rows whose every logit is masked with the type's lowest value) the
+// difference is taken first.
+__device__ __forceinline__ bool far(float m) { return fabsf(m) > 1e30f; }
+__device__ __forceinline__ float term(float x, float m, float c) {
+  return far(m) ? (x - m) * c : fmaf(x, c, -__fmul_rn(m, c));
+}
+// What a sum relative to `from` is multiplied with to be relative to `to`, both
+// the largest logits of parts of a row, from <= to. A part without a logit above
+// -inf has the lowest number as its largest: its sum is 0 (or NaN) and stays so.
+__device__ __forceinline__ float rebase(float from, float to, float c) {
+  const float a = (from - to) * c, b = __fmul_rn(from, c) - __fmul_rn(to, c);
+  return exp2_fast(far(to) ? a : b);
+}
+
 // One 16-byte piece of a row: 4 fp32 or 8 bf16 values.
 template <class T>
 struct Piece {
   static constexpr int N = 16 / sizeof(T);
-  uint32_t w[4];
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void none() {  // -inf everywhere
+    const uint32_t v = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+    w = make_uint4(v, v, v, v);
+  }
   __device__ __forceinline__ float get(int i) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    else return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[i]);
+    else return __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
   }
-  // Elements [first, first + N) of a row of V elements at z; elements outside
-  // the row read as -inf. z + first is 16-byte aligned.
-  __device__ __forceinline__ void load(const T* z, int first, int V) {
-    if (first >= 0 && first + N <= V) {
-      const uint4 v = *reinterpret_cast<const uint4*>(z + first);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;  // -inf
-    if (first >= V) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = first + i;
-      if (e < 0 || e >= V) continue;
-      if constexpr (sizeof(T) == 4) {
-        w[i] = __float_as_uint(z[e]);
-      } else {
-        const uint32_t b = *reinterpret_cast<const unsigned short*>(z + e);
-        w[i >> 1] = i & 1 ? (w[i >> 1] & 0xFFFFu) | (b << 16) : (w[i >> 1] & 0xFFFF0000u) | b;
-      }
-    }
-  }
-  // Store v[0..N) to elements [first, first + N) of the row d of V elements, as
-  // one 16-byte store where `wide` says that d + first is 16-byte aligned.
-  static __device__ __forceinline__ void store(T* d, int first, int V, const float* v, bool wide) {
-    if (wide && first >= 0 && first + N <= V) {
+  static __device__ __forceinline__ void store(T* p, const float* v, bool wide) {
+    if (wide) {
       uint4 o;
       if constexpr (sizeof(T) == 4) {
         o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
@@ -104,21 +110,52 @@ struct Piece {
         for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
         o = *reinterpret_cast<const uint4*>(h);
       }
-      *reinterpret_cast<uint4*>(d + first) = o;
-      return;
-    }
+      *reinterpret_cast<uint4*>(p) = o;
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (first + i >= 0 && first + i < V) from_f(d + first + i, v[i]);
+      for (int i = 0; i < N; ++i) from_f(p + i, v[i]);
+    }
   }
 };
 
-// Elements of z that lie before its first 16-byte boundary, counted from the
-// boundary below: element e of the row sits at place e + phase(z) of a 16-byte
-// grid.
-template <class T>
-__device__ __forceinline__ int phase(const T* z) {
-  return (int)(((uintptr_t)z & 15) / sizeof(T));
+// The largest value of a thread's pieces, at least the lowest number (bf16: two
+// at a time; NaN is ignored, the sum of exponentials finds it).
+template <int NP>
+__device__ __forceinline__ float piece_max(const Piece<float>* x) {
+  float m = -FLT_MAX;
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, x[j].get(i));
+  return m;
 }
+template <int NP>
+__device__ __forceinline__ float piece_max(const Piece<__nv_bfloat16>* x) {
+  auto h = [](uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+  __nv_bfloat162 m = h(0xFF80FF80u);
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+    m = __hmax2(m, __hmax2(__hmax2(h(x[j].w.x), h(x[j].w.y)), __hmax2(h(x[j].w.z), h(x[j].w.w))));
+  return fmaxf(fmaxf(__low2float(m), __high2float(m)), -FLT_MAX);
+}
+
+// How a row of V elements at z lies on the 16-byte grid: `head` elements before
+// the first boundary, `pieces` whole pieces, then the rest. The at most
+// 2 (N - 1) elements outside the pieces are edge elements, one a thread.
+template <class T>
+struct Grid {
+  int head, pieces, V;
+  __device__ __forceinline__ Grid(const T* z, int v) : V(v) {
+    constexpr int N = Piece<T>::N;
+    head = min((N - (int)(((uintptr_t)z & 15) / sizeof(T))) & (N - 1), v);
+    pieces = (v - head) / N;
+  }
+  __device__ __forceinline__ int at(int piece) const { return head + piece * Piece<T>::N; }
+  // edge element i, or -1
+  __device__ __forceinline__ int edge(int i) const {
+    const int e = i < head ? i : at(pieces) + i - head;
+    return e < V ? e : -1;
+  }
+};
 
 }  // namespace rnet_logits

@@ -77,10 +77,11 @@ __global__ void __launch_bounds__(LT) topk_kernel(const T* __restrict__ logits, 
 // ---------------------------------------------------------------- distillation
 // L = w [ soft tau^2 sum_k p_k (log p_k - log q_ik) + hard (lse_1 - z_y) ],
 // q = softmax(z / tau), and dL/dz = w [ soft tau (P q - p) + hard (softmax(z) -
-// 1_y) ] with P = sum p. A row is read once and held in registers: its maximum
-// and sum of exponentials, then the gradient of every element without the
-// record, then the at most K + 1 elements that a record or label touches once
-// more. What bounds it is HBM: one read and one write of the logits.
+// 1_y) ] with P = sum p. A row is read once; its exponentials, relative to the
+// thread's own maximum, stay in registers until the row's sum is known and then
+// only need a factor. The at most K + 1 elements that a record or label touches
+// are written a second time. What bounds it is HBM: one read and one write of
+// the logits.
 struct DistillArgs {
   const int* t_idx;
   const float* t_val;
@@ -95,395 +96,462 @@ struct DistillArgs {
 
 // What a row's gradient needs beside its elements.
 struct RowGrad {
-  float m;        // largest logit
-  float c;        // log2(e) / tau
-  float a, a1;    // factors of 2^((x - m) c) and of 2^((x - m) log2(e))
-  float pf, hf;   // what a unit of teacher probability and the label take off
+  float m;      // largest logit
+  float c;      // log2(e) / tau
+  float a, a1;  // factors of 2^term(x, m, c) and of 2^term(x, m, log2(e))
+  float pf, hf; // what a unit of teacher probability and the label take off
   template <bool HARD>
   __device__ __forceinline__ float at(float x) const {
-    const float d = x - m;
-    float v = a * exp2_fast(d * c);
-    if (HARD) v += a1 * exp2_fast(d * LOG2E);
+    float v = a * exp2_fast(term(x, m, c));
+    if (HARD) v += a1 * exp2_fast(term(x, m, LOG2E));
     return v;
   }
 };
 
-// The record of one row in shared memory, filled by one warp.
+// The record and label of one row, held by one warp: entry k in lane k % 32.
+template <int J>
 struct Record {
-  int idx[RNET_TOPK_MAX];
-  float p[RNET_TOPK_MAX];
-  float lp[RNET_TOPK_MAX];  // log p
-  float z[RNET_TOPK_MAX];
-  int target;
-  float z_target;
-  float P;         // sum p
-  int has_target;  // the label is one of the entries
-  int twice;       // an index may come more than once
+  int idx[J];  // -1: no entry
+  float z[J], p[J], lp[J];  // student's logit, teacher's probability and its log
+  int y;       // label, -1: none
+  float zy;
+  float P;     // sum p
+  bool bad;    // this lane saw an index beyond the vocabulary
+
+  // First the loads that depend on nothing, then the student's logits at the
+  // indices.
+  __device__ __forceinline__ void read(size_t row, const DistillArgs& a) {
+    const int lane = threadIdx.x & 31;
+    y = a.hard != 0.f ? a.targets[row] : -1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int k = lane + 32 * j;
+      const bool in = k < a.K && a.soft != 0.f;
+      idx[j] = in ? a.t_idx[row * a.K + k] : -1;
+      lp[j] = in ? a.t_val[row * a.K + k] : -INFINITY;
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void gather(const T* row, int V) {
+    bad = y >= V;
+    if (bad) y = -1;
+    zy = y >= 0 ? to_f(row[y]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (idx[j] >= V) bad = true, idx[j] = -1;
+      z[j] = idx[j] >= 0 ? to_f(row[idx[j]]) : 0.f;
+    }
+  }
+  // Probabilities relative to the record's own maximum, or to the teacher's
+  // normaliser if it is given. An entry at -inf has none.
+  __device__ __forceinline__ void weigh(size_t row, const DistillArgs& a) {
+    float tm = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      lp[j] = idx[j] >= 0 ? lp[j] * a.inv_tau : -INFINITY;
+      tm = fmaxf(tm, lp[j]);
+    }
+    const bool given = a.t_lse != nullptr;
+    const float shift = given ? a.t_lse[row] : warp_max(tm);
+    float S = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bool none = lp[j] == -INFINITY;
+      lp[j] -= shift;
+      p[j] = none ? 0.f : exp2_fast(lp[j] * LOG2E);
+      S += p[j];
+    }
+    P = warp_sum(S);
+    if (given || P == 0.f) return;
+    const float inv = __fdividef(1.0f, P), ln = LN2 * log2_fast(P);
+#pragma unroll
+    for (int j = 0; j < J; ++j) p[j] *= inv, lp[j] -= ln;
+    P *= inv;
+  }
+  // This lane's part of sum p (log p - term).
+  __device__ __forceinline__ float kl(float m, float c) const {
+    float v = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (p[j] != 0.f) v += p[j] * (lp[j] - LN2 * term(z[j], m, c));
+    return v;
+  }
+  // The row's loss from sum p (log p - term) and the sums of 2^term.
+  __device__ __forceinline__ float loss(const DistillArgs& a, float w, float kl, float m, float s,
+                                        float s1) const {
+    if (s == 0.f) return 0.f;  // every logit -inf: no distribution
+    float l = 0.f;
+    if (a.soft != 0.f) {
+      if (P != 0.f) kl += P * (LN2 * log2_fast(s));
+      l = a.soft * a.tau * a.tau * kl;
+    }
+    if (y >= 0) l += a.hard * (LN2 * (log2_fast(s1) - term(zy, m, LOG2E)));
+    return w * l;
+  }
+  // The record's and the label's elements, those that are `in` this CTA's share,
+  // once more with their own terms, after the stores of the whole share.
+  template <bool HARD, class T, class In>
+  __device__ __forceinline__ void fix(T* d, const RowGrad& g, int K, In in) const {
+    const int lane = threadIdx.x & 31;
+    bool hot = false, twice = J > 1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) hot |= y >= 0 && idx[j] == y;
+    if (J == 1)
+      twice = __any_sync(~0u, (__match_any_sync(~0u, idx[0] < 0 ? ~lane : idx[0]) &
+                               ~(1u << lane)) != 0);
+    float sum[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) sum[j] = p[j];
+    if (twice) {  // the same index may come more than once: all its parts, in order
+#pragma unroll
+      for (int j = 0; j < J; ++j) sum[j] = 0.f;
+#pragma unroll
+      for (int h = 0; h < J; ++h)
+        for (int k = 0; k < 32 && k + 32 * h < K; ++k) {
+          const int i = __shfl_sync(~0u, idx[h], k);
+          const float v = __shfl_sync(~0u, p[h], k);
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            if (idx[j] == i) sum[j] += v;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (idx[j] >= 0 && in(idx[j])) {
+        float v = g.at<HARD>(z[j]) - g.pf * sum[j];
+        if (HARD && idx[j] == y) v -= g.hf;
+        from_f(d + idx[j], v);
+      }
+    if (HARD && !__any_sync(~0u, hot) && lane == 0 && y >= 0 && in(y))
+      from_f(d + y, g.at<HARD>(zy) - g.hf);
+  }
 };
 
-// Reads a row's record and label (one warp). Probabilities relative to the
-// record's own maximum, or to the teacher's normaliser if it is given.
-template <class T>
-__device__ __forceinline__ void read_record(Record& r, const T* z, size_t row,
-                                            const DistillArgs& a, bool report) {
-  constexpr int J = RNET_TOPK_MAX / 32;
-  const int lane = threadIdx.x & 31;
-  int y = -1;
-  if (a.hard != 0.f) y = a.targets[row];
-  bool bad = y >= a.V;
-  if (bad) y = -1;
-  float t[J];
-  float tm = -INFINITY;
-  bool hot = false, twice = a.K > 32;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int k = lane + 32 * j;
-    t[j] = -INFINITY;
-    if (32 * j >= a.K) break;
-    int i = -1;
-    if (k < a.K && a.soft != 0.f) i = a.t_idx[row * a.K + k];
-    if (i >= a.V) bad = true, i = -1;
-    if (i >= 0) {
-      t[j] = a.t_val[row * a.K + k] * a.inv_tau;
-      r.z[k] = to_f(z[i]);
-      hot |= i == y;
-    }
-    if (k < a.K) r.idx[k] = i;
-    tm = fmaxf(tm, t[j]);
-    if (j == 0 && !twice)
-      twice = __any_sync(~0u, (__match_any_sync(~0u, i < 0 ? ~lane : i) & ~(1u << lane)) != 0);
-  }
-  const float shift = a.t_lse ? a.t_lse[row] : warp_max(tm);
-  float S = 0.f;
-  float d[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    // an entry at -inf (padding reads as one) has no probability
-    d[j] = t[j] - shift;
-    t[j] = t[j] == -INFINITY ? 0.f : expf(d[j]);
-    S += t[j];
-  }
-  S = warp_sum(S);
-  const bool given = a.t_lse != nullptr;
-  const float norm = given || S == 0.f ? 1.0f : 1.0f / S;
-  const float ln = given || S == 0.f ? 0.f : logf(S);
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-    if (lane + 32 * j < a.K) {
-      r.p[lane + 32 * j] = t[j] * norm;
-      r.lp[lane + 32 * j] = d[j] - ln;
-    }
-  hot = __any_sync(~0u, hot);
-  if (lane == 0) {
-    r.target = y;
-    r.z_target = y >= 0 ? to_f(z[y]) : 0.f;
-    r.P = S * norm;
-    r.has_target = hot;
-    r.twice = twice;
-  }
-  if (bad && report && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
-}
-
 // Gradient factors from the row's maximum m and its sums s (at tau) and s1 (at
-// 1) of 2^((x - m) ...).
-__device__ __forceinline__ RowGrad row_factors(const Record& r, const DistillArgs& a, float w,
+// 1) of 2^term. The quotients are within 2 ulp.
+__device__ __forceinline__ RowGrad row_factors(float P, bool label, const DistillArgs& a, float w,
                                                float m, float s, float s1) {
   RowGrad g;
-  const bool none = m == -INFINITY && s == 0.f;  // every logit -inf: no distribution
-  const bool label = r.target >= 0;
+  const bool none = s == 0.f;  // every logit -inf: no distribution
   const float gw = none ? 0.f : w * a.scale;
-  g.m = none ? 0.f : m;
+  g.m = m;
   g.c = a.inv_tau * LOG2E;
   g.pf = a.soft != 0.f ? gw * a.soft * a.tau : 0.f;
   g.hf = label ? gw * a.hard : 0.f;
-  g.a = none || a.soft == 0.f ? 0.f : g.pf * r.P / s;
-  g.a1 = none || !label ? 0.f : g.hf / s1;
+  g.a = none || a.soft == 0.f ? 0.f : g.pf * __fdividef(P, s);
+  g.a1 = none || !label ? 0.f : g.hf * __fdividef(1.0f, s1);
   return g;
 }
 
-// The row's loss (one warp; the result in every lane).
-__device__ __forceinline__ float row_loss(const Record& r, const DistillArgs& a, float w, float m,
-                                          float s, float s1) {
-  if (m == -INFINITY && s == 0.f) return 0.f;
-  float loss = 0.f;
-  if (a.soft != 0.f) {
-    float kl = 0.f;
-    for (int k = threadIdx.x & 31; k < a.K; k += 32)
-      if (r.p[k] != 0.f) kl += r.p[k] * (r.lp[k] - (r.z[k] - m) * a.inv_tau);
-    kl = warp_sum(kl);
-    if (r.P != 0.f) kl += r.P * logf(s);
-    loss = a.soft * a.tau * a.tau * kl;
-  }
-  if (r.target >= 0) loss += a.hard * ((m - r.z_target) + logf(s1));
-  return w * loss;
-}
+// A thread's share of a row: E elements in pieces, and one edge element.
+template <class T, int E, bool HARD>
+struct Share {
+  static constexpr int N = Piece<T>::N, NP = E / N;
+  float e[E + 1];
+  float e1[HARD ? E + 1 : 1];
+  float m, s, s1;  // largest logit and sums, relative to it
 
-// Element i of the record (i == K: the label) once more, with its own terms.
-template <class T, bool HARD>
-__device__ __forceinline__ void fix_entry(T* d, int i, const Record& r, const RowGrad& g, int K,
-                                          int lo, int hi) {
-  if (i == K && r.has_target) return;
-  const int e = i < K ? r.idx[i] : r.target;
-  if (e < lo || e >= hi) return;
-  float p = i < K ? r.p[i] : 0.f;
-  if (r.twice) {
-    p = 0.f;
-    for (int k = 0; k < K; ++k)
-      if (r.idx[k] == e) p += r.p[k];
+  __device__ __forceinline__ void take(const Piece<T>* x, float edge, float c) {
+    m = fmaxf(piece_max<NP>(x), edge);
+    s = s1 = 0.f;
+    const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
+    if (far(m)) {
+      fill(x, edge, [&](float v) { return (v - m) * c; }, [&](float v) { return (v - m) * LOG2E; });
+    } else {
+      fill(x, edge, [&](float v) { return fmaf(v, c, -mc); },
+           [&](float v) { return fmaf(v, LOG2E, -m1); });
+    }
   }
-  float v = g.at<HARD>(i < K ? r.z[i] : r.z_target) - g.pf * p;
-  if (HARD && e == r.target) v -= g.hf;
-  from_f(d + e, v);
+  template <class F, class F1>
+  __device__ __forceinline__ void fill(const Piece<T>* x, float edge, F t, F1 t1) {
+#pragma unroll
+    for (int i = 0; i <= E; ++i) {
+      const float v = i < E ? x[i / N].get(i % N) : edge;
+      e[i] = exp2_fast(t(v));
+      s += e[i];
+      if (HARD) {
+        e1[i] = exp2_fast(t1(v));
+        s1 += e1[i];
+      }
+    }
+  }
+  // e * f (+ e1 * f1): the gradient of every element, to the pieces q0 + j * step
+  // below q1 and to the edge element
+  __device__ __forceinline__ void write(T* d, const Grid<T>& grid, int q0, int step, int q1,
+                                        int edge, float f, float f1) const {
+    auto grad = [&](int i) { return HARD ? fmaf(f1, e1[i], f * e[i]) : f * e[i]; };
+    T* p = d + grid.at(q0);
+    auto all = [&](bool wide) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = grad(j * N + i);
+        if (q0 + j * step < q1) Piece<T>::store(p + j * step * N, v, wide);
+      }
+    };
+    if (((uintptr_t)p & 15) == 0) all(true);
+    else all(false);  // the logits and their gradient lie differently on the 16-byte grid
+    if (edge >= 0) from_f(d + edge, grad(E));
+  }
+};
+
+// The pieces q0 + j * step below q1 of a row.
+template <class T, int NP>
+__device__ __forceinline__ void load_pieces(Piece<T>* x, const T* z, const Grid<T>& grid, int q0,
+                                            int step, int q1) {
+  const T* p = z + grid.at(q0);
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    x[j].none();
+    if (q0 + j * step < q1) x[j].load(p + j * step * Piece<T>::N);
+  }
+}
+template <class T>
+__device__ __forceinline__ void zero_pieces(T* d, const Grid<T>& grid, int q0, int step, int q1,
+                                            int edge) {
+  const float zero[Piece<T>::N] = {};
+  for (int q = q0; q < q1; q += step)
+    Piece<T>::store(d + grid.at(q), zero, ((uintptr_t)(d + grid.head) & 15) == 0);
+  if (edge >= 0) from_f(d + edge, 0.f);
 }
 
 constexpr int WARPS = 8;  // rows of a CTA of the warp-per-row kernel
 
-// Up to 32 * NP pieces of 16 bytes: a warp per row, the row in registers.
-template <class T, int NP, bool HARD>
-__global__ void __launch_bounds__(32 * WARPS) distill_warp_kernel(
+// Rows of up to 32 * E elements in pieces: a warp per row.
+template <class T, int E, int J, bool HARD>
+__global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 4 : 2) distill_warp_kernel(
     const T* logits, long long ld, T* dlogits, long long ldd, DistillArgs a, int rows) {
   rnet_dev::pdl_trigger();
-  constexpr int N = Piece<T>::N;
-  __shared__ Record rec[WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t row = (size_t)blockIdx.x * WARPS + warp;
+  constexpr int N = Piece<T>::N, NP = E / N;
+  const int lane = threadIdx.x & 31;
+  const size_t row = (size_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const T* z = logits + row * ld;
-  T* d = dlogits ? dlogits + row * ldd : nullptr;
-  const int V = a.V, ph = phase(z);
-  const bool wide = d && phase(d) == ph;
   const float w = a.weight ? a.weight[row] : 1.0f;
+  Record<J> r;
+  r.read(row, a);
+  const T* z = logits + row * ld;
+  const Grid<T> grid(z, a.V);
+  const int edge = grid.edge(lane);
+  Piece<T> x[NP];
+  load_pieces<T, NP>(x, z, grid, lane, 32, grid.pieces);
+  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+  T* d = dlogits ? dlogits + row * ldd : nullptr;
   if (w == 0.f) {  // whatever the row holds
-    const float zero[N] = {};
-    if (d)
-      for (int j = 0; j < NP; ++j) Piece<T>::store(d, (lane + 32 * j) * N - ph, V, zero, wide);
+    if (d) zero_pieces(d, grid, lane, 32, grid.pieces, edge);
     if (lane == 0) a.row_loss[row] = 0.f;
     return;
   }
-  Piece<T> x[NP];
-#pragma unroll
-  for (int j = 0; j < NP; ++j) x[j].load(z, (lane + 32 * j) * N - ph, V);
-  Record& r = rec[warp];
-  read_record(r, z, row, a, true);
-  float m = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < NP; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, x[j].get(i));
-  m = warp_max(m);
-  const float ms = m == -INFINITY ? 0.f : m, c = a.inv_tau * LOG2E;
-  float s = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int j = 0; j < NP; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float e = x[j].get(i) - ms;
-      s += exp2_fast(e * c);
-      if (HARD) s1 += exp2_fast(e * LOG2E);
-    }
-  s = warp_sum(s);
-  if (HARD) s1 = warp_sum(s1);
-  __syncwarp();
-  const float loss = row_loss(r, a, w, m, s, s1);
-  if (lane == 0) a.row_loss[row] = loss;
+  r.gather(z, a.V);
+  const float c = a.inv_tau * LOG2E;
+  Share<T, E, HARD> h;
+  h.take(x, xe, c);
+  r.weigh(row, a);
+  const float m = warp_max(h.m);
+  const float f = rebase(h.m, m, c), f1 = HARD ? rebase(h.m, m, LOG2E) : 0.f;
+  const float s = warp_sum(h.s * f), s1 = HARD ? warp_sum(h.s1 * f1) : 0.f;
+  const float kl = warp_sum(r.kl(m, c));
+  if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
+  if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   if (!d) return;
-  const RowGrad g = row_factors(r, a, w, m, s, s1);
-#pragma unroll
-  for (int j = 0; j < NP; ++j) {
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = g.at<HARD>(x[j].get(i));
-    Piece<T>::store(d, (lane + 32 * j) * N - ph, V, v, wide);
-  }
+  const RowGrad g = row_factors(r.P, r.y >= 0, a, w, m, s, s1);
+  __syncwarp();  // the reads of the row come before the stores, where dlogits are the logits
+  h.write(d, grid, lane, 32, grid.pieces, edge, g.a * f, g.a1 * f1);
   __syncwarp();  // orders the stores above before those below
-  for (int i = lane; i <= a.K; i += 32) fix_entry<T, HARD>(d, i, r, g, a.K, 0, V);
+  r.template fix<HARD>(d, g, a.K, [](int) { return true; });
 }
 
-__device__ __forceinline__ void store_remote(float* p, uint32_t rank, float v) {
+__device__ __forceinline__ void store_remote(float4* p, uint32_t rank, float4 v) {
   asm volatile(
       "{\n\t.reg .b32 ra;\n\t"
       "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
-      "st.shared::cluster.f32 [ra], %2;\n\t}" ::"r"(rnet_dev::smem_u32(p)),
-      "r"(rank), "f"(v)
+      "st.shared::cluster.v4.f32 [ra], {%2, %3, %4, %5};\n\t}" ::"r"(rnet_dev::smem_u32(p)),
+      "r"(rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
       : "memory");
 }
 
-// Longer rows: a cluster of C = 1, 2, 4 or 8 CTAs per row, each with up to
-// THREADS * NP pieces in registers. The CTAs' maxima and sums meet through
-// distributed shared memory and are joined in rank order, so every CTA uses the
-// same bits.
-template <class T, int THREADS, int NP, bool HARD>
+constexpr int CLUSTER = 16;  // CTAs of one row at most
+
+// Longer rows: a cluster of C CTAs per row, each with up to THREADS * E
+// elements. Every warp leaves its maximum and sums in the shared memory of all
+// CTAs of the cluster, and joins them all in the same order: one exchange, and
+// the same bits everywhere. Warp 0 of each CTA holds the record.
+template <class T, int THREADS, int E, int J, bool HARD>
 __global__ void __launch_bounds__(THREADS) distill_cta_kernel(const T* logits, long long ld,
                                                               T* dlogits, long long ldd,
-                                                              DistillArgs a, int C) {
+                                                              DistillArgs a, int per) {
   rnet_dev::pdl_trigger();
-  constexpr int N = Piece<T>::N, NW = THREADS / 32;
-  __shared__ Record r;
-  __shared__ float part[NW][3];
-  __shared__ float joint[8][3];
+  constexpr int N = Piece<T>::N, NP = E / N, NW = THREADS / 32;
+  __shared__ float4 part[CLUSTER * NW];  // m, s, s1
+  __shared__ float s_P;
+  __shared__ int s_label;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const size_t row = blockIdx.x / C;
-  const int rank = blockIdx.x % C;
-  const T* z = logits + row * ld;
-  T* d = dlogits ? dlogits + row * ldd : nullptr;
-  const int V = a.V, ph = phase(z);
-  const bool wide = d && phase(d) == ph;
-  const int pieces = (V + ph + N - 1) / N, per = (pieces + C - 1) / C;
-  const int begin = rank * per, end = min(begin + per, pieces);
-  auto first = [&](int j) {  // V: no element
-    const int q = begin + tid + j * THREADS;
-    return q < end ? q * N - ph : V;
-  };
+  const size_t row = blockIdx.x;
+  const int rank = blockIdx.y, C = gridDim.y;
   const float w = a.weight ? a.weight[row] : 1.0f;
+  Record<J> r;
+  if (warp == 0) r.read(row, a);
+  const T* z = logits + row * ld;
+  const Grid<T> grid(z, a.V);
+  const int begin = rank * per, end = min(begin + per, grid.pieces);
+  const int edge = rank == 0 && tid < 2 * N ? grid.edge(tid) : -1;  // the first CTA's
+  Piece<T> x[NP];
+  load_pieces<T, NP>(x, z, grid, begin + tid, THREADS, end);
+  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+  T* d = dlogits ? dlogits + row * ldd : nullptr;
   if (w == 0.f) {  // whatever the row holds; the whole cluster leaves
-    const float zero[N] = {};
-    if (d)
-      for (int j = 0; j < NP; ++j) Piece<T>::store(d, first(j), V, zero, wide);
+    if (d) zero_pieces(d, grid, begin + tid, THREADS, end, edge);
     if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
     return;
   }
   // the peers' shared memory may be written once all of them run
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  Piece<T> x[NP];
-#pragma unroll
-  for (int j = 0; j < NP; ++j) x[j].load(z, first(j), V);
-  if (warp == 0) read_record(r, z, row, a, rank == 0);
+  if (warp == 0) r.gather(z, a.V);
   const float c = a.inv_tau * LOG2E;
-  float m = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < NP; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, x[j].get(i));
-  const float m0 = m == -INFINITY ? 0.f : m;
-  float s = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int j = 0; j < NP; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float e = x[j].get(i) - m0;
-      s += exp2_fast(e * c);
-      if (HARD) s1 += exp2_fast(e * LOG2E);
-    }
-  // relative to the warp's maximum, the CTA's, the row's (a part without a
-  // logit above -inf has sums of 0, or of NaN, and keeps them)
-  auto rebase = [&](float to, float from, float& v, float& v1) {
-    const float e = from == -INFINITY ? 0.f : from - to;
-    v *= exp2_fast(e * c);
-    if (HARD) v1 *= exp2_fast(e * LOG2E);
-  };
-  const float mw = warp_max(m);
-  rebase(mw, m, s, s1);
-  s = warp_sum(s);
-  if (HARD) s1 = warp_sum(s1);
-  if (lane == 0) part[warp][0] = mw, part[warp][1] = s, part[warp][2] = s1;
-  __syncthreads();
-  m = -INFINITY;
-  for (int i = 0; i < NW; ++i) m = fmaxf(m, part[i][0]);
-  s = s1 = 0.f;
-  for (int i = 0; i < NW; ++i) {
-    float v = part[i][1], v1 = part[i][2];
-    rebase(m, part[i][0], v, v1);
-    s += v, s1 += v1;
+  Share<T, E, HARD> h;
+  h.take(x, xe, c);
+  if (warp == 0) {
+    r.weigh(row, a);
+    if (lane == 0) s_P = r.P, s_label = r.y >= 0;
+    if (r.bad && rank == 0 && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   }
+  float m = warp_max(h.m);
+  float s = warp_sum(h.s * rebase(h.m, m, c));
+  float s1 = HARD ? warp_sum(h.s1 * rebase(h.m, m, LOG2E)) : 0.f;
+  const float4 mine = make_float4(m, s, s1, 0.f);
   if (C > 1) {
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (tid < C) {
-      store_remote(&joint[rank][0], tid, m);
-      store_remote(&joint[rank][1], tid, s);
-      store_remote(&joint[rank][2], tid, s1);
-    }
+    if (lane < C) store_remote(&part[rank * NW + warp], lane, mine);
     rnet_dev::cluster_sync();
-    m = -INFINITY;
-    for (int i = 0; i < C; ++i) m = fmaxf(m, joint[i][0]);
-    s = s1 = 0.f;
-    for (int i = 0; i < C; ++i) {
-      float v = joint[i][1], v1 = joint[i][2];
-      rebase(m, joint[i][0], v, v1);
-      s += v, s1 += v1;
-    }
+  } else {
+    if (lane == 0) part[warp] = mine;
+    __syncthreads();
   }
+  constexpr int MOST = NW == 8 ? 2 : CLUSTER * NW / 32;  // 256 threads: at most 8 CTAs
+  float4 got[MOST];
+  m = -FLT_MAX;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    got[i] = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
+    if (lane + 32 * i < C * NW) got[i] = part[lane + 32 * i];
+    m = fmaxf(m, got[i].x);
+  }
+  m = warp_max(m);
+  s = s1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    s += got[i].y * rebase(got[i].x, m, c);
+    if (HARD) s1 += got[i].z * rebase(got[i].x, m, LOG2E);
+  }
+  s = warp_sum(s);
+  if (HARD) s1 = warp_sum(s1);
   if (rank == 0 && warp == 0) {
-    const float loss = row_loss(r, a, w, m, s, s1);
-    if (lane == 0) a.row_loss[row] = loss;
+    const float kl = warp_sum(r.kl(m, c));
+    if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;
-  const RowGrad g = row_factors(r, a, w, m, s, s1);
-#pragma unroll
-  for (int j = 0; j < NP; ++j) {
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = g.at<HARD>(x[j].get(i));
-    Piece<T>::store(d, first(j), V, v, wide);
-  }
+  const RowGrad g = row_factors(s_P, s_label, a, w, m, s, s1);
+  h.write(d, grid, begin + tid, THREADS, end, edge, g.a * rebase(h.m, m, c),
+          HARD ? g.a1 * rebase(h.m, m, LOG2E) : 0.f);
   __syncthreads();  // orders the stores above before those below
-  const int lo = max(begin * N - ph, 0), hi = min(end * N - ph, V);
-  for (int i = tid; i <= a.K; i += THREADS) fix_entry<T, HARD>(d, i, r, g, a.K, lo, hi);
+  if (warp == 0) {
+    const int lo = grid.at(begin), hi = grid.at(max(begin, end));
+    const int head = grid.head, tail = grid.at(grid.pieces);
+    r.template fix<HARD>(d, g, a.K, [&](int e) {
+      return (e >= lo && e < hi) || (rank == 0 && (e < head || e >= tail));
+    });
+  }
 }
 
-template <class T, int THREADS, int NP, bool HARD>
+template <class T, int THREADS, int E, int J, bool HARD>
 cudaError_t distill_cta(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                         int rows, int C, cudaStream_t s) {
-  if ((long long)rows * C > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kernel = distill_cta_kernel<T, THREADS, E, J, HARD>;
+  if (C > 8) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows * C);
+  cfg.gridDim = dim3(rows, C);
   cfg.blockDim = dim3(THREADS);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.y = C;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, distill_cta_kernel<T, THREADS, NP, HARD>, z, ld, d, ldd, a, C);
+  return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a,
+                            (a.V / Piece<T>::N + C - 1) / C);
 }
 
-template <class T, bool HARD>
+template <class T, int J, bool HARD>
 cudaError_t distill_launch(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                            int rows, cudaStream_t s) {
-  constexpr int N = Piece<T>::N;
-  // places before a row's first element, at most
-  const int ph = ((size_t)z | (size_t)ld * sizeof(T)) % 16 ? N - 1 : 0;
-  const int pieces = (a.V + ph + N - 1) / N;
+  const int V = a.V;  // at least the elements in pieces
   const int grid = (rows + WARPS - 1) / WARPS, block = 32 * WARPS;
-  if (pieces <= 32)
-    distill_warp_kernel<T, 1, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
-  else if (pieces <= 64)
-    distill_warp_kernel<T, 2, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
-  else if (pieces <= 128)
-    distill_warp_kernel<T, 4, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
-  else {
-    // the fewest CTAs of 256 threads that hold the row, 8 pieces a thread;
-    // more of them while they leave SMs idle
-    int C = 1;
-    while (C < 8 && 256 * 8 * C < pieces) C *= 2;
-    while (C < 8 && rows * C < 148 && 256 * C < pieces) C *= 2;
-    const int per = (pieces + C - 1) / C;
-    if (per <= 256) return distill_cta<T, 256, 1, HARD>(z, ld, d, ldd, a, rows, C, s);
-    if (per <= 512) return distill_cta<T, 256, 2, HARD>(z, ld, d, ldd, a, rows, C, s);
-    if (per <= 1024) return distill_cta<T, 256, 4, HARD>(z, ld, d, ldd, a, rows, C, s);
-    if (per <= 2048) return distill_cta<T, 256, 8, HARD>(z, ld, d, ldd, a, rows, C, s);
-    if (per <= 4096) return distill_cta<T, 512, 8, HARD>(z, ld, d, ldd, a, rows, C, s);
-    // the limit of the vocabulary, in an unaligned row
-    constexpr int LAST = RNET_DISTILL_VOCAB_MAX / 8 / 1024 / N + 1;
-    if (per <= 1024 * LAST) return distill_cta<T, 1024, LAST, HARD>(z, ld, d, ldd, a, rows, C, s);
-    return cudaErrorInvalidValue;
+  if (V <= 32 * 8)
+    distill_warp_kernel<T, 8, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+  else if (V <= 32 * 16)
+    distill_warp_kernel<T, 16, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+  else if (V <= 32 * 32)
+    distill_warp_kernel<T, 32, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+  else if (V <= 8 * 256 * 32) {
+    // the fewest CTAs that hold the row at 32 elements a thread, or more of
+    // them, with fewer elements each, while they leave SMs idle
+    int C = (V + 256 * 32 - 1) / (256 * 32);
+    while (C < 8 && (long long)rows * (C + 1) <= 148 && C * 256 * 8 < V) ++C;
+    const int per = ((V + C - 1) / C + 7) & ~7;
+    if (per <= 256 * 8) return distill_cta<T, 256, 8, J, HARD>(z, ld, d, ldd, a, rows, C, s);
+    if (per <= 256 * 16) return distill_cta<T, 256, 16, J, HARD>(z, ld, d, ldd, a, rows, C, s);
+    return distill_cta<T, 256, 32, J, HARD>(z, ld, d, ldd, a, rows, C, s);
+  } else {
+    const int C = (V + 512 * 32 - 1) / (512 * 32);
+    if (C > CLUSTER) return cudaErrorInvalidValue;
+    return distill_cta<T, 512, 32, J, HARD>(z, ld, d, ldd, a, rows, C, s);
   }
   return cudaGetLastError();
 }
 
+// Sum of the rows' losses in 64 bits, in a fixed order. Launched so that it may
+// start while the last rows are still at work, and then waits for all of them.
 __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* __restrict__ x, int n,
                                                         float* __restrict__ out) {
+  __shared__ double sh[32];
+  rnet_dev::pdl_wait();
   rnet_dev::pdl_trigger();
-  __shared__ double sh[1024];
   double a = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) a += x[i];
-  sh[threadIdx.x] = a;
-  __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
-    __syncthreads();
+  int i = threadIdx.x;
+  for (; i + 7 * 1024 < n; i += 8 * 1024) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = x[i + j * 1024];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a += v[j];
   }
-  if (threadIdx.x == 0) *out = (float)sh[0];
+  for (; i < n; i += 1024) a += x[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  a = sh[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+  if (threadIdx.x == 0) *out = (float)a;
+}
+
+cudaError_t sum_rows(const float* x, int n, float* out, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sum_rows_kernel, x, n, out);
 }
 
 }  // namespace
@@ -507,24 +575,23 @@ cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int*
   DistillArgs a{t_idx, t_val, t_lse, targets, weight, 1.0f / tau, tau, soft, hard, scale, row_loss,
                 err, V, K};
   if (rows > 0) {
-    cudaError_t e;
-    if (bf16) {
-      const __nv_bfloat16* z = (const __nv_bfloat16*)logits;
-      __nv_bfloat16* d = (__nv_bfloat16*)dlogits;
-      e = hard != 0.f ? distill_launch<__nv_bfloat16, true>(z, ld, d, ldd, a, rows, s)
-                      : distill_launch<__nv_bfloat16, false>(z, ld, d, ldd, a, rows, s);
-    } else {
-      const float* z = (const float*)logits;
-      float* d = (float*)dlogits;
-      e = hard != 0.f ? distill_launch<float, true>(z, ld, d, ldd, a, rows, s)
-                      : distill_launch<float, false>(z, ld, d, ldd, a, rows, s);
-    }
+    auto run = [&](auto type) {
+      using T = decltype(type);
+      const T* z = (const T*)logits;
+      T* d = (T*)dlogits;
+      if (hard != 0.f)
+        return K > 32 ? distill_launch<T, 2, true>(z, ld, d, ldd, a, rows, s)
+                      : distill_launch<T, 1, true>(z, ld, d, ldd, a, rows, s);
+      return K > 32 ? distill_launch<T, 2, false>(z, ld, d, ldd, a, rows, s)
+                    : distill_launch<T, 1, false>(z, ld, d, ldd, a, rows, s);
+    };
+    const cudaError_t e = bf16 ? run(__nv_bfloat16()) : run(0.0f);
     if (e != cudaSuccess) return e;
     launched();
   }
   if (!loss) return cudaSuccess;
-  sum_rows_kernel<<<1, 1024, 0, s>>>(row_loss, rows, loss);
-  return launched();
+  const cudaError_t e = sum_rows(row_loss, rows, loss, s);
+  return e != cudaSuccess ? e : launched();
 }
 
 }  // namespace rnet_k
