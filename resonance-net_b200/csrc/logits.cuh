@@ -8,6 +8,8 @@
 #include <cfloat>
 #include <cstdint>
 
+#include "common.cuh"
+
 namespace rnet_logits {
 
 __device__ __forceinline__ float to_f(float x) { return x; }
@@ -157,5 +159,16 @@ struct Grid {
     return e < V ? e : -1;
   }
 };
+
+// Copy of `bytes` (a multiple of 16, both ends 16-byte aligned) to shared
+// memory; its arrival counts on the barrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(rnet_dev::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(rnet_dev::smem_u32(bar))
+      : "memory");
+}
 
 }  // namespace rnet_logits

@@ -1,5 +1,7 @@
 // Records of a row's largest logits, and the distillation loss against such
 // records with its gradient.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
@@ -361,79 +363,18 @@ __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 4 : 2) dist
   r.template fix<HARD>(d, g, a.K, [](int) { return true; });
 }
 
-__device__ __forceinline__ void store_remote(float4* p, uint32_t rank, float4 v) {
-  asm volatile(
-      "{\n\t.reg .b32 ra;\n\t"
-      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
-      "st.shared::cluster.v4.f32 [ra], {%2, %3, %4, %5};\n\t}" ::"r"(rnet_dev::smem_u32(p)),
-      "r"(rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-      : "memory");
-}
-
-constexpr int CLUSTER = 16;  // CTAs of one row at most
-
-// Longer rows: a cluster of C CTAs per row, each with up to THREADS * E
-// elements. Every warp leaves its maximum and sums in the shared memory of all
-// CTAs of the cluster, and joins them all in the same order: one exchange, and
-// the same bits everywhere. Warp 0 of each CTA holds the record.
-template <class T, int THREADS, int E, int J, bool HARD>
-__global__ void __launch_bounds__(THREADS) distill_cta_kernel(const T* logits, long long ld,
-                                                              T* dlogits, long long ldd,
-                                                              DistillArgs a, int per) {
-  rnet_dev::pdl_trigger();
-  constexpr int N = Piece<T>::N, NP = E / N, NW = THREADS / 32;
-  __shared__ float4 part[CLUSTER * NW];  // m, s, s1
-  __shared__ float s_P;
-  __shared__ int s_label;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const size_t row = blockIdx.x;
-  const int rank = blockIdx.y, C = gridDim.y;
-  const float w = a.weight ? a.weight[row] : 1.0f;
-  Record<J> r;
-  if (warp == 0) r.read(row, a);
-  const T* z = logits + row * ld;
-  const Grid<T> grid(z, a.V);
-  const int begin = rank * per, end = min(begin + per, grid.pieces);
-  const int edge = rank == 0 && tid < 2 * N ? grid.edge(tid) : -1;  // the first CTA's
-  Piece<T> x[NP];
-  load_pieces<T, NP>(x, z, grid, begin + tid, THREADS, end);
-  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
-  T* d = dlogits ? dlogits + row * ldd : nullptr;
-  if (w == 0.f) {  // whatever the row holds; the whole cluster leaves
-    if (d) zero_pieces(d, grid, begin + tid, THREADS, end, edge);
-    if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
-    return;
-  }
-  // the peers' shared memory may be written once all of them run
-  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (warp == 0) r.gather(z, a.V);
-  const float c = a.inv_tau * LOG2E;
-  Share<T, E, HARD> h;
-  h.take(x, xe, c);
-  if (warp == 0) {
-    r.weigh(row, a);
-    if (lane == 0) s_P = r.P, s_label = r.y >= 0;
-    if (r.bad && rank == 0 && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
-  }
-  float m = warp_max(h.m);
-  float s = warp_sum(h.s * rebase(h.m, m, c));
-  float s1 = HARD ? warp_sum(h.s1 * rebase(h.m, m, LOG2E)) : 0.f;
-  const float4 mine = make_float4(m, s, s1, 0.f);
-  if (C > 1) {
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (lane < C) store_remote(&part[rank * NW + warp], lane, mine);
-    rnet_dev::cluster_sync();
-  } else {
-    if (lane == 0) part[warp] = mine;
-    __syncthreads();
-  }
-  constexpr int MOST = NW == 8 ? 2 : CLUSTER * NW / 32;  // 256 threads: at most 8 CTAs
+// A row's maximum and sums from the parts (m, s, s1) of n warps, joined in the
+// same order by every warp.
+template <int MOST, bool HARD>
+__device__ __forceinline__ void join_parts(const float4* part, int n, float c, float& m, float& s,
+                                           float& s1) {
+  const int lane = threadIdx.x & 31;
   float4 got[MOST];
   m = -FLT_MAX;
 #pragma unroll
   for (int i = 0; i < MOST; ++i) {
     got[i] = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
-    if (lane + 32 * i < C * NW) got[i] = part[lane + 32 * i];
+    if (lane + 32 * i < n) got[i] = part[lane + 32 * i];
     m = fmaxf(m, got[i].x);
   }
   m = warp_max(m);
@@ -445,17 +386,220 @@ __global__ void __launch_bounds__(THREADS) distill_cta_kernel(const T* logits, l
   }
   s = warp_sum(s);
   if (HARD) s1 = warp_sum(s1);
+}
+
+// Rows of up to 256 * E elements in pieces: a CTA per row, the row in
+// registers. Warp 0 holds the record.
+template <class T, int E, int J, bool HARD>
+__global__ void __launch_bounds__(256) distill_cta_kernel(const T* logits, long long ld,
+                                                          T* dlogits, long long ldd,
+                                                          DistillArgs a) {
+  rnet_dev::pdl_trigger();
+  constexpr int N = Piece<T>::N, NP = E / N;
+  __shared__ float4 part[8];
+  __shared__ float s_P;
+  __shared__ int s_label;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const size_t row = blockIdx.x;
+  const float w = a.weight ? a.weight[row] : 1.0f;
+  Record<J> r;
+  if (warp == 0) r.read(row, a);
+  const T* z = logits + row * ld;
+  const Grid<T> grid(z, a.V);
+  const int edge = tid < 2 * N ? grid.edge(tid) : -1;
+  Piece<T> x[NP];
+  load_pieces<T, NP>(x, z, grid, tid, 256, grid.pieces);
+  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+  T* d = dlogits ? dlogits + row * ldd : nullptr;
+  if (w == 0.f) {  // whatever the row holds
+    if (d) zero_pieces(d, grid, tid, 256, grid.pieces, edge);
+    if (tid == 0) a.row_loss[row] = 0.f;
+    return;
+  }
+  if (warp == 0) r.gather(z, a.V);
+  const float c = a.inv_tau * LOG2E;
+  Share<T, E, HARD> h;
+  h.take(x, xe, c);
+  if (warp == 0) {
+    r.weigh(row, a);
+    if (lane == 0) s_P = r.P, s_label = r.y >= 0;
+    if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
+  }
+  float m = warp_max(h.m);
+  float s = warp_sum(h.s * rebase(h.m, m, c));
+  float s1 = HARD ? warp_sum(h.s1 * rebase(h.m, m, LOG2E)) : 0.f;
+  if (lane == 0) part[warp] = make_float4(m, s, s1, 0.f);
+  __syncthreads();
+  join_parts<1, HARD>(part, 8, c, m, s, s1);
+  if (warp == 0) {
+    const float kl = warp_sum(r.kl(m, c));
+    if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
+  }
+  if (!d) return;
+  const RowGrad g = row_factors(s_P, s_label, a, w, m, s, s1);
+  h.write(d, grid, tid, 256, grid.pieces, edge, g.a * rebase(h.m, m, c),
+          HARD ? g.a1 * rebase(h.m, m, LOG2E) : 0.f);
+  __syncthreads();  // orders the stores above before those below
+  if (warp == 0) r.template fix<HARD>(d, g, a.K, [](int) { return true; });
+}
+
+__device__ __forceinline__ void store_remote(float4* p, uint32_t rank, float4 v) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "st.shared::cluster.v4.f32 [ra], {%2, %3, %4, %5};\n\t}" ::"r"(rnet_dev::smem_u32(p)),
+      "r"(rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+      : "memory");
+}
+
+constexpr int CLUSTER = 8;      // CTAs of one row at most
+constexpr int LONG = 512;       // their threads
+constexpr int CHUNK = 4 * LONG; // pieces (32 KB) that arrive together
+constexpr int CHUNKS = 5;
+// Pieces of a row in one CTA's shared memory, so that two CTAs share an SM and
+// one reads while the other computes and writes.
+constexpr int SHARE = 108 * 1024 / 16;
+static_assert(RNET_DISTILL_VOCAB_MAX * 4 / 16 <= CLUSTER * CHUNK * CHUNKS, "vocab limit");
+
+// Longer rows: a cluster of C CTAs per row, each with `per` pieces in shared
+// memory. Chunks of the row arrive by bulk copies, and their maxima and sums are
+// taken as they do. Every warp leaves its own in the shared memory of all CTAs of
+// the cluster: one exchange, and the same bits everywhere. The gradient is then
+// computed from shared memory. Warp 0 of each CTA holds the record.
+template <class T, int J, bool HARD>
+__global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, long long ld,
+                                                               T* dlogits, long long ldd,
+                                                               DistillArgs a, int per) {
+  rnet_dev::pdl_trigger();
+  constexpr int N = Piece<T>::N, NW = LONG / 32;
+  extern __shared__ uint4 long_buf[];
+  Piece<T>* const buf = reinterpret_cast<Piece<T>*>(long_buf);
+  __shared__ float4 part[CLUSTER * NW];  // m, s, s1
+  __shared__ __align__(8) uint64_t bar[CHUNKS];
+  __shared__ float s_P;
+  __shared__ int s_label, s_abort[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const size_t row = blockIdx.x;
+  const int rank = blockIdx.y, C = gridDim.y;
+  const T* z = logits + row * ld;
+  const Grid<T> grid(z, a.V);
+  const int begin = min(rank * per, grid.pieces), n = min(per, grid.pieces - begin);
+  if (tid == 0) {
+    s_abort[0] = s_abort[1] = 0;
+    for (int i = 0; i < CHUNKS; ++i) rnet_dev::mbar_init(&bar[i], 1);
+    rnet_dev::fence_barrier_init();
+    for (int i = 0; i * CHUNK < n; ++i) {
+      const uint32_t bytes = 16u * min(CHUNK, n - i * CHUNK);
+      rnet_dev::mbar_arrive_expect_tx(&bar[i], bytes);
+      bulk_load(buf + i * CHUNK, z + grid.at(begin + i * CHUNK), bytes, &bar[i]);
+    }
+  }
+  // the peers' shared memory may be written once all of them run
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const float w = a.weight ? a.weight[row] : 1.0f;
+  Record<J> r;
+  if (warp == 0) r.read(row, a);
+  const int edge = rank == 0 && tid < 2 * N ? grid.edge(tid) : -1;  // the first CTA's
+  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+  T* d = dlogits ? dlogits + row * ldd : nullptr;
+  const float c = a.inv_tau * LOG2E;
+  if (warp == 0) {
+    r.gather(z, a.V);
+    r.weigh(row, a);
+    if (lane == 0) s_P = r.P, s_label = r.y >= 0;
+    if (r.bad && rank == 0 && w != 0.f && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
+  }
+  __syncthreads();  // the barriers are set up
+  float m = -FLT_MAX, s = 0.f, s1 = 0.f;
+  auto add = [&](float mx, auto each) {
+    s *= rebase(m, mx, c);
+    if (HARD) s1 *= rebase(m, mx, LOG2E);
+    m = mx;
+    const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
+    if (far(m)) {
+      each([&](float v) {
+        s += exp2_fast((v - m) * c);
+        if (HARD) s1 += exp2_fast((v - m) * LOG2E);
+      });
+    } else {
+      each([&](float v) {
+        s += exp2_fast(fmaf(v, c, -mc));
+        if (HARD) s1 += exp2_fast(fmaf(v, LOG2E, -m1));
+      });
+    }
+  };
+  if (edge >= 0) add(fmaxf(m, xe), [&](auto f) { f(xe); });
+  for (int i = 0; i * CHUNK < n; ++i) {
+    // a copy that does not come is reported and given the same time once more:
+    // none may land in memory that the CTA has left
+    if (!rnet_dev::mbar_wait(&bar[i], 0, a.err, &s_abort[0]))
+      rnet_dev::mbar_wait(&bar[i], 0, a.err, &s_abort[1]);
+    Piece<T> x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int q = i * CHUNK + j * LONG + tid;
+      x[j].none();
+      if (q < n) x[j] = buf[q];
+    }
+    add(fmaxf(m, piece_max<4>(x)), [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < N; ++k) f(x[j].get(k));
+    });
+  }
+  {
+    const float mw = warp_max(m);
+    s = warp_sum(s * rebase(m, mw, c));
+    if (HARD) s1 = warp_sum(s1 * rebase(m, mw, LOG2E));
+    m = mw;
+  }
+  const float4 mine = make_float4(m, s, s1, 0.f);
+  if (C > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (lane < C) store_remote(&part[rank * NW + warp], lane, mine);
+    rnet_dev::cluster_sync();
+  } else {
+    if (lane == 0) part[warp] = mine;
+    __syncthreads();
+  }
+  if (w == 0.f) {  // whatever the row holds
+    if (d) zero_pieces(d, grid, begin + tid, LONG, begin + n, edge);
+    if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
+    return;
+  }
+  join_parts<CLUSTER * NW / 32, HARD>(part, C * NW, c, m, s, s1);
   if (rank == 0 && warp == 0) {
     const float kl = warp_sum(r.kl(m, c));
     if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;
   const RowGrad g = row_factors(s_P, s_label, a, w, m, s, s1);
-  h.write(d, grid, begin + tid, THREADS, end, edge, g.a * rebase(h.m, m, c),
-          HARD ? g.a1 * rebase(h.m, m, LOG2E) : 0.f);
+  T* p = d + grid.at(begin);
+  auto write = [&](bool wide, auto value) {
+#pragma unroll 2
+    for (int q = tid; q < n; q += LONG) {
+      const Piece<T> x = buf[q];
+      float v[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = value(x.get(k));
+      Piece<T>::store(p + (size_t)q * N, v, wide);
+    }
+  };
+  const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
+  auto near_value = [&](float v) {
+    const float e = g.a * exp2_fast(fmaf(v, c, -mc));
+    return HARD ? fmaf(g.a1, exp2_fast(fmaf(v, LOG2E, -m1)), e) : e;
+  };
+  if (far(m) || ((uintptr_t)p & 15))
+    // also where logits and gradient lie differently on the 16-byte grid
+    write(((uintptr_t)p & 15) == 0, [&](float v) { return g.template at<HARD>(v); });
+  else
+    write(true, near_value);
+  if (edge >= 0) from_f(d + edge, g.template at<HARD>(xe));
   __syncthreads();  // orders the stores above before those below
   if (warp == 0) {
-    const int lo = grid.at(begin), hi = grid.at(max(begin, end));
+    const int lo = grid.at(begin), hi = grid.at(begin + n);
     const int head = grid.head, tail = grid.at(grid.pieces);
     r.template fix<HARD>(d, g, a.K, [&](int e) {
       return (e >= lo && e < hi) || (rank == 0 && (e < head || e >= tail));
@@ -463,17 +607,31 @@ __global__ void __launch_bounds__(THREADS) distill_cta_kernel(const T* logits, l
   }
 }
 
-template <class T, int THREADS, int E, int J, bool HARD>
-cudaError_t distill_cta(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
-                        int rows, int C, cudaStream_t s) {
-  auto kernel = distill_cta_kernel<T, THREADS, E, J, HARD>;
-  if (C > 8) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+template <class T, int J, bool HARD>
+cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
+                         int rows, cudaStream_t s) {
+  auto kernel = distill_long_kernel<T, J, HARD>;
+  const int pieces = a.V / Piece<T>::N;
+  int C = (pieces + SHARE - 1) / SHARE;
+  // more CTAs while they would leave SMs idle and have two chunks each
+  while (C < CLUSTER && (long long)rows * (C + 1) <= 148 && pieces / (C + 1) >= 2 * LONG) ++C;
+  if (C > CLUSTER) C = CLUSTER;
+  const int per = (pieces + C - 1) / C;
+  if (per > CHUNK * CHUNKS) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> ready{0};  // devices whose limit is raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             16 * CHUNK * CHUNKS);
     if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows, C);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(LONG);
+  cfg.dynamicSmemBytes = (size_t)per * 16;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -481,8 +639,7 @@ cudaError_t distill_cta(const T* z, long long ld, T* d, long long ldd, const Dis
   at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a,
-                            (a.V / Piece<T>::N + C - 1) / C);
+  return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a, per);
 }
 
 template <class T, int J, bool HARD>
@@ -496,20 +653,14 @@ cudaError_t distill_launch(const T* z, long long ld, T* d, long long ldd, const 
     distill_warp_kernel<T, 16, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
   else if (V <= 32 * 32)
     distill_warp_kernel<T, 32, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
-  else if (V <= 8 * 256 * 32) {
-    // the fewest CTAs that hold the row at 32 elements a thread, or more of
-    // them, with fewer elements each, while they leave SMs idle
-    int C = (V + 256 * 32 - 1) / (256 * 32);
-    while (C < 8 && (long long)rows * (C + 1) <= 148 && C * 256 * 8 < V) ++C;
-    const int per = ((V + C - 1) / C + 7) & ~7;
-    if (per <= 256 * 8) return distill_cta<T, 256, 8, J, HARD>(z, ld, d, ldd, a, rows, C, s);
-    if (per <= 256 * 16) return distill_cta<T, 256, 16, J, HARD>(z, ld, d, ldd, a, rows, C, s);
-    return distill_cta<T, 256, 32, J, HARD>(z, ld, d, ldd, a, rows, C, s);
-  } else {
-    const int C = (V + 512 * 32 - 1) / (512 * 32);
-    if (C > CLUSTER) return cudaErrorInvalidValue;
-    return distill_cta<T, 512, 32, J, HARD>(z, ld, d, ldd, a, rows, C, s);
-  }
+  else if (V <= 256 * 8)
+    distill_cta_kernel<T, 8, J, HARD><<<rows, 256, 0, s>>>(z, ld, d, ldd, a);
+  else if (V <= 256 * 16)
+    distill_cta_kernel<T, 16, J, HARD><<<rows, 256, 0, s>>>(z, ld, d, ldd, a);
+  else if (V <= 256 * 32)
+    distill_cta_kernel<T, 32, J, HARD><<<rows, 256, 0, s>>>(z, ld, d, ldd, a);
+  else
+    return distill_long<T, J, HARD>(z, ld, d, ldd, a, rows, s);
   return cudaGetLastError();
 }
 
