@@ -3,101 +3,205 @@
 #include "common.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
+#include "select.cuh"
 
 namespace rnet_k {
 namespace {
 
 using namespace rnet_logits;
 
-constexpr int BT = 256;
-
-struct Cand {
-  double total;
-  unsigned long long flat;  // beam * vocab + token
+// ---------------------------------------------------------------- selection
+// The best `beams` of score[b] + z[b][v] - lse[b] over (b, v): within a row the
+// order of the totals is that of the logits, so each row (or slice of a row)
+// gives its W largest logits and its sum of exponentials, and one warp merges
+// the sorted lists, a lane each. Totals are formed and compared in 64 bits.
+// What bounds it is HBM for long rows, latency for short ones.
+struct SelectArgs {
+  const float* scores_in;
+  const int* finished_in;
+  int eos;
+  float* scores;
+  int *tokens, *parents, *finished;
+  int W, V;
 };
-__device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-  return a.total > b.total || (a.total == b.total && a.flat < b.flat);
+
+// A list per (beam, slice), in that order, so that of equal totals the lowest
+// lane's is the lowest candidate.
+struct Lists {
+  uint64_t key[RNET_BEAMS_MAX][RNET_BEAMS_MAX];
+  double s[RNET_BEAMS_MAX];
+  float m[RNET_BEAMS_MAX];
+  int n[RNET_BEAMS_MAX];
+};
+
+__device__ __forceinline__ uint64_t order(double x) {
+  const int64_t b = __double_as_longlong(x);
+  return (uint64_t)b ^ ((uint64_t)(b >> 63) | 0x8000000000000000ull);
 }
 
-// One CTA per sequence: the log-normaliser of each beam's row, then `beams`
-// rounds, each finding the best candidate after the last one.
-template <class T>
-__global__ void __launch_bounds__(BT) beam_select_kernel(
-    const T* __restrict__ logits, long long ld, const float* scores_in, const int* finished_in,
-    int eos, float* scores, int* tokens, int* parents, int* finished, int W, int V) {
-  rnet_dev::pdl_trigger();
-  __shared__ double s_lse[RNET_BEAMS_MAX], s_score[RNET_BEAMS_MAX];
-  __shared__ int s_done[RNET_BEAMS_MAX];
-  __shared__ double shd[BT / 32];
-  __shared__ float shf[BT / 32];
-  __shared__ Cand shc[BT / 32];
-  const size_t m0 = (size_t)blockIdx.x * W;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < W) {
-    s_score[threadIdx.x] = canon(scores_in[m0 + threadIdx.x]);
-    s_done[threadIdx.x] = finished_in ? finished_in[m0 + threadIdx.x] != 0 : 0;
-  }
-  for (int b = 0; b < W; ++b) {
-    const T* z = logits + (m0 + b) * ld;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < V; i += BT) m = fmaxf(m, canon(to_f(z[i])));
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if (lane == 0) shf[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < BT / 32; ++i) m = fmaxf(m, shf[i]);
-    double s = 0.0;
-    if (m > -INFINITY)
-      for (int i = threadIdx.x; i < V; i += BT) s += expf(canon(to_f(z[i])) - m);
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    if (lane == 0) shd[warp] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s = 0.0;
-      for (int i = 0; i < BT / 32; ++i) s += shd[i];
-      s_lse[b] = m + log(s);
+// One warp: W rounds over the heads of the W * S lists.
+__device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size_t m0, int S) {
+  const int lane = threadIdx.x & 31, W = a.W;
+  const int beam = lane / S, part = lane % S;
+  const bool on = lane < W * S;
+  double score = -INFINITY, lse = 0.0;
+  bool done = false;
+  int n = 0;
+  if (on) {
+    score = canon(a.scores_in[m0 + beam]);
+    done = a.finished_in && a.finished_in[m0 + beam];
+    if (done) {
+      n = part == 0;  // (beam, eos) at its own score
+    } else {
+      n = in.n[lane];
+      float m = in.m[beam * S];
+      for (int i = 1; i < S; ++i) m = fmaxf(m, in.m[beam * S + i]);
+      double s = 0.0;
+      for (int i = 0; i < S; ++i)
+        s += in.s[beam * S + i] * (double)exp2_fast((in.m[beam * S + i] - m) * LOG2E);
+      lse = log_sum(m, s, 1.0f);
     }
-    __syncthreads();
   }
-  Cand last{INFINITY, 0};
+  __syncwarp();  // every input is read before the outputs, which may be the inputs
+  int at = 0, token = 0;
+  double total = -INFINITY;
+  auto next = [&]() {
+    total = -INFINITY;
+    if (at >= n) return;
+    if (done) {
+      token = a.eos;
+      total = score;
+    } else {
+      const uint64_t k = in.key[lane][at];
+      token = key_index(k);
+      total = score + ((double)key_value(k) - lse);
+    }
+    ++at;
+  };
+  next();
   for (int j = 0; j < W; ++j) {
-    Cand best{-INFINITY, ~0ull};
-    for (int b = 0; b < W; ++b) {
-      const T* z = logits + (m0 + b) * ld;
-      const unsigned long long f0 = (unsigned long long)b * V;
-      if (s_done[b]) {
-        const Cand c{s_score[b], f0 + eos};
-        if (threadIdx.x == 0 && better(last, c) && better(c, best)) best = c;
-        continue;
-      }
-      for (int i = threadIdx.x; i < V; i += BT) {
-        const float x = canon(to_f(z[i]));
-        if (x == -INFINITY) continue;
-        const Cand c{s_score[b] + ((double)x - s_lse[b]), f0 + i};
-        if (better(last, c) && better(c, best)) best = c;
-      }
+    const uint64_t o = order(total);
+    const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(o >> 32));
+    const bool top = (uint32_t)(o >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(~0u, top ? (uint32_t)o : 0u);
+    const int win = __ffs(__ballot_sync(~0u, top && (uint32_t)o == lo)) - 1;
+    const bool live = __shfl_sync(~0u, total, win) > -INFINITY;
+    const bool stays = __shfl_sync(~0u, done, (j * S) & 31);
+    if (live ? lane == win : lane == 0) {
+      const int t = live ? token : a.eos >= 0 ? a.eos : 0;
+      a.scores[m0 + j] = live ? (float)total : -INFINITY;
+      a.parents[m0 + j] = live ? beam : j;
+      a.tokens[m0 + j] = t;
+      if (a.finished) a.finished[m0 + j] = (live ? done : stays) || t == a.eos;
     }
-    for (int o = 16; o; o >>= 1) {
-      const Cand c{__shfl_xor_sync(~0u, best.total, o), __shfl_xor_sync(~0u, best.flat, o)};
-      if (better(c, best)) best = c;
-    }
-    if (lane == 0) shc[warp] = best;
-    __syncthreads();
-    for (int i = 0; i < BT / 32; ++i)
-      if (better(shc[i], best)) best = shc[i];
-    __syncthreads();
-    last = best;
-    if (threadIdx.x == 0) {
-      const bool live = best.total > -INFINITY;
-      const int parent = live ? (int)(best.flat / V) : j;
-      const int token = live ? (int)(best.flat % V) : (eos >= 0 ? eos : 0);
-      scores[m0 + j] = live ? (float)best.total : -INFINITY;
-      parents[m0 + j] = parent;
-      tokens[m0 + j] = token;
-      if (finished) finished[m0 + j] = s_done[parent] || token == eos;
-    }
+    if (live && lane == win) next();
   }
 }
 
+// Rows of up to 32 * R words: a CTA per sequence, a warp per beam.
+template <class T, int R>
+__global__ void __launch_bounds__(32 * RNET_BEAMS_MAX) beam_select_warps_kernel(
+    const T* __restrict__ logits, long long ld, SelectArgs a) {
+  rnet_dev::pdl_trigger();
+  __shared__ Lists lists;
+  extern __shared__ uint64_t keys[];  // WARP_CAP a warp
+  const int lane = threadIdx.x & 31, beam = threadIdx.x >> 5;
+  const size_t m0 = (size_t)blockIdx.x * a.W;
+  const T* z = logits + (m0 + beam) * ld;
+  const bool even = even_start(z);
+  uint32_t w[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) w[j] = load_word(z, lane + 32 * j, a.V, even);
+  uint64_t* own = keys + beam * WARP_CAP;
+  float m;
+  double s;
+  const int n = warp_select<T, R>(w, a.W, LOG2E, own, m, s);
+  if (lane < n) lists.key[beam][lane] = own[lane];
+  if (lane == 0) lists.n[beam] = n, lists.m[beam] = m, lists.s[beam] = s;
+  __syncthreads();
+  if (beam == 0) merge(lists, a, m0, 1);
+}
+
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+  uint32_t ra;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(ra) : "r"(rnet_dev::smem_u32(p)));
+  return ra;
+}
+__device__ __forceinline__ void store_u64(uint32_t ra, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ra), "l"(v) : "memory");
+}
+__device__ __forceinline__ void store_u32(uint32_t ra, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ra), "r"(v) : "memory");
+}
+
+// Longer rows: a cluster per sequence. The W * S (beam, slice) parts go round the
+// CTAs of the cluster; their lists meet in the first CTA's shared memory.
+template <class T>
+__global__ void __launch_bounds__(SEL_THREADS) beam_select_cluster_kernel(
+    const T* __restrict__ logits, long long ld, SelectArgs a, int S, int slice) {
+  rnet_dev::pdl_trigger();
+  __shared__ Lists lists;
+  __shared__ Selection sel;
+  const int tid = threadIdx.x, rank = blockIdx.y, C = gridDim.y;
+  const size_t m0 = (size_t)blockIdx.x * a.W;
+  // the first CTA's shared memory may be written once it runs
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  bool waited = C == 1;
+  for (int u = rank; u < a.W * S; u += C) {
+    const int beam = u / S, begin = (u % S) * slice, end = min(begin + slice, a.V);
+    float m = 0.f;
+    double s = 0.0;
+    int n = 0;
+    if (!(a.finished_in && a.finished_in[m0 + beam]))
+      n = cta_select(sel, logits + (m0 + beam) * ld, min(begin, a.V), end, a.W, LOG2E, m, s);
+    if (!waited) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    waited = true;
+    if (tid < n) store_u64(in_first_cta(&lists.key[u][tid]), sel.key[tid]);
+    if (tid == 0) {
+      store_u32(in_first_cta(&lists.n[u]), n);
+      store_u32(in_first_cta(&lists.m[u]), __float_as_uint(m));
+      store_u64(in_first_cta(&lists.s[u]), (uint64_t)__double_as_longlong(s));
+    }
+    __syncthreads();  // sel is free again
+  }
+  if (C > 1) rnet_dev::cluster_sync();
+  if (rank == 0 && tid < 32) merge(lists, a, m0, S);
+}
+
+template <class T>
+cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int batch,
+                          cudaStream_t s) {
+  constexpr int N = Words<T>::N;
+  const int block = 32 * a.W;
+  const size_t smem = (size_t)a.W * WARP_CAP * sizeof(uint64_t);
+  if (a.V <= 256) {
+    beam_select_warps_kernel<T, 8 / N><<<batch, block, smem, s>>>(z, ld, a);
+    return cudaGetLastError();
+  }
+  if (a.V <= 1024) {
+    beam_select_warps_kernel<T, 32 / N><<<batch, block, smem, s>>>(z, ld, a);
+    return cudaGetLastError();
+  }
+  // slices of a row where the rows alone leave SMs idle, one pass or more each
+  int S = 1;
+  const int pass = SEL_THREADS * SEL_R * N;
+  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * pass < a.V) ++S;
+  const int slice = (((a.V + S - 1) / S) + 1) & ~1;
+  const int C = a.W * S < 8 ? a.W * S : 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(batch, C);
+  cfg.blockDim = dim3(SEL_THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.y = C;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1;
+  return cudaLaunchKernelEx(&cfg, beam_select_cluster_kernel<T>, z, ld, a, S, slice);
+}
+
+// ---------------------------------------------------------------- states
 // Rows [outer][batch][beams] of `row` vectors: dst row j of a group is src row
 // parents[j]. A thread owns one vector column of a group: it reads the parents'
 // values of every beam before it writes any, so dst may be src.
@@ -193,14 +297,10 @@ cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float
                         const int* finished_in, int eos, float* scores, int* tokens, int* parents,
                         int* finished, int batch, int beams, int V, cudaStream_t s) {
   if (batch <= 0) return cudaSuccess;
-  if (bf16)
-    beam_select_kernel<<<batch, BT, 0, s>>>((const __nv_bfloat16*)logits, ld, scores_in,
-                                            finished_in, eos, scores, tokens, parents, finished,
-                                            beams, V);
-  else
-    beam_select_kernel<<<batch, BT, 0, s>>>((const float*)logits, ld, scores_in, finished_in, eos,
-                                            scores, tokens, parents, finished, beams, V);
-  return launched();
+  const SelectArgs a{scores_in, finished_in, eos, scores, tokens, parents, finished, beams, V};
+  const cudaError_t e = bf16 ? select_launch((const __nv_bfloat16*)logits, ld, a, batch, s)
+                             : select_launch((const float*)logits, ld, a, batch, s);
+  return e != cudaSuccess ? e : launched();
 }
 
 cudaError_t beam_reorder(const void* src, void* dst, size_t row_bytes, size_t pitch, size_t outer,

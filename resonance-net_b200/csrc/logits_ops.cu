@@ -5,75 +5,80 @@
 #include "common.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
+#include "select.cuh"
 
 namespace rnet_k {
 namespace {
 
 using namespace rnet_logits;
 
-constexpr int LT = 256;  // threads per row
+// ---------------------------------------------------------------- records
+// One pass over the row for its K largest logits and its sum of exponentials.
+// What bounds it is HBM for long rows, and the instructions of the selection for
+// short ones.
+struct TopkArgs {
+  float c, inv_tau;
+  float* top;
+  int* idx;
+  float* lse;
+  int V, K;
+};
 
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int i = 1; i < LT / 32; ++i) v = fmaxf(v, sh[i]);
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < LT / 32; ++i) v += sh[i];
-  __syncthreads();
-  return v;
+__device__ __forceinline__ void write_place(const TopkArgs& a, size_t row, int k, bool in,
+                                            uint64_t key) {
+  a.top[row * a.K + k] = in ? key_value(key) : -INFINITY;
+  a.idx[row * a.K + k] = in ? key_index(key) : -1;
 }
 
-// One CTA per row; K rounds, each finds the largest key below the last one.
-template <class T>
-__global__ void __launch_bounds__(LT) topk_kernel(const T* __restrict__ logits, long long ld,
-                                                  float inv_tau, float* __restrict__ top,
-                                                  int* __restrict__ idx, float* __restrict__ lse,
-                                                  int V, int K) {
+constexpr int TOPK_WARPS = 4;
+
+// Rows of up to 32 * R words: a warp per row.
+template <class T, int R>
+__global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __restrict__ logits,
+                                                                    long long ld, TopkArgs a,
+                                                                    int rows) {
   rnet_dev::pdl_trigger();
-  __shared__ float sh[LT / 32];
-  __shared__ uint64_t shk[LT / 32];
-  const T* z = logits + (size_t)blockIdx.x * ld;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += LT) m = fmaxf(m, canon(to_f(z[i])));
-  m = block_max(m, sh);
-  if (lse) {
-    float s = 0.f;
-    if (m > -INFINITY)
-      for (int i = threadIdx.x; i < V; i += LT) s += expf((canon(to_f(z[i])) - m) * inv_tau);
-    s = block_sum(s, sh);
-    if (threadIdx.x == 0) lse[blockIdx.x] = m > -INFINITY ? m * inv_tau + logf(s) : -INFINITY;
-  }
-  uint64_t below = ~0ull;
-  for (int k = 0; k < K; ++k) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < V; i += LT) {
-      const float x = canon(to_f(z[i]));
-      const uint64_t key = make_key(x, i);
-      if (x > -INFINITY && key < below && key > best) best = key;
-    }
-    for (int o = 16; o; o >>= 1) {
-      const uint64_t b = __shfl_xor_sync(~0u, best, o);
-      best = b > best ? b : best;
-    }
-    if ((threadIdx.x & 31) == 0) shk[threadIdx.x >> 5] = best;
-    __syncthreads();
-    for (int i = 0; i < LT / 32; ++i) best = shk[i] > best ? shk[i] : best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      top[(size_t)blockIdx.x * K + k] = best ? key_value(best) : -INFINITY;
-      idx[(size_t)blockIdx.x * K + k] = best ? key_index(best) : -1;
-    }
-    below = best;
-  }
+  __shared__ uint64_t keys[TOPK_WARPS][WARP_CAP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t row = (size_t)blockIdx.x * TOPK_WARPS + warp;
+  if (row >= rows) return;
+  const T* z = logits + row * ld;
+  const bool even = even_start(z);
+  uint32_t w[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) w[j] = load_word(z, lane + 32 * j, a.V, even);
+  float m;
+  double s;
+  const int n = warp_select<T, R>(w, a.K, a.c, keys[warp], m, s);
+  for (int k = lane; k < a.K; k += 32) write_place(a, row, k, k < n, keys[warp][k]);
+  if (lane == 0 && a.lse) a.lse[row] = (float)log_sum(m, s, a.inv_tau);
+}
+
+// Longer rows: a CTA per row.
+template <class T>
+__global__ void __launch_bounds__(SEL_THREADS) topk_cta_kernel(const T* __restrict__ logits,
+                                                               long long ld, TopkArgs a) {
+  rnet_dev::pdl_trigger();
+  __shared__ Selection sel;
+  const size_t row = blockIdx.x;
+  float m;
+  double s;
+  const int n = cta_select(sel, logits + row * ld, 0, a.V, a.K, a.c, m, s);
+  if (threadIdx.x < a.K)
+    write_place(a, row, threadIdx.x, threadIdx.x < n, sel.key[threadIdx.x]);
+  if (threadIdx.x == 0 && a.lse) a.lse[row] = (float)log_sum(m, s, a.inv_tau);
+}
+
+template <class T>
+void topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
+  constexpr int N = Words<T>::N;
+  const int grid = (rows + TOPK_WARPS - 1) / TOPK_WARPS, block = 32 * TOPK_WARPS;
+  if (a.V <= 256)
+    topk_warp_kernel<T, 8 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
+  else if (a.V <= 1024)
+    topk_warp_kernel<T, 32 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
+  else
+    topk_cta_kernel<T><<<rows, SEL_THREADS, 0, s>>>(z, ld, a);
 }
 
 // ---------------------------------------------------------------- distillation
@@ -710,11 +715,9 @@ cudaError_t sum_rows(const float* x, int n, float* out, cudaStream_t s) {
 cudaError_t topk_logits(const void* logits, bool bf16, long long ld, float tau, float* top,
                         int* idx, float* lse, int rows, int V, int K, cudaStream_t s) {
   if (rows <= 0) return cudaSuccess;
-  if (bf16)
-    topk_kernel<<<rows, LT, 0, s>>>((const __nv_bfloat16*)logits, ld, 1.0f / tau, top, idx, lse, V,
-                                    K);
-  else
-    topk_kernel<<<rows, LT, 0, s>>>((const float*)logits, ld, 1.0f / tau, top, idx, lse, V, K);
+  const TopkArgs a{LOG2E / tau, 1.0f / tau, top, idx, lse, V, K};
+  if (bf16) topk_launch((const __nv_bfloat16*)logits, ld, a, rows, s);
+  else topk_launch((const float*)logits, ld, a, rows, s);
   return launched();
 }
 
