@@ -23,6 +23,7 @@ struct SelectArgs {
   float* scores;
   int *tokens, *parents, *finished;
   int W, V;
+  unsigned* err;
 };
 
 // A list per (beam, slice), in that order, so that of equal totals the lowest
@@ -59,7 +60,7 @@ __device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size
       double s = 0.0;
       for (int i = 0; i < S; ++i)
         s += in.s[beam * S + i] * (double)exp2_fast((in.m[beam * S + i] - m) * LOG2E);
-      lse = log_sum(m, s, 1.0f);
+      lse = log_sum(m, s);
     }
   }
   __syncwarp();  // every input is read before the outputs, which may be the inputs
@@ -99,8 +100,8 @@ __device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size
 }
 
 // Rows of up to 32 * R words: a CTA per sequence, a warp per beam.
-template <class T, int R>
-__global__ void __launch_bounds__(32 * RNET_BEAMS_MAX) beam_select_warps_kernel(
+template <class T, int R, int MOST>
+__global__ void __launch_bounds__(32 * MOST) beam_select_warps_kernel(
     const T* __restrict__ logits, long long ld, SelectArgs a) {
   rnet_dev::pdl_trigger();
   __shared__ Lists lists;
@@ -141,19 +142,23 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_select_cluster_kernel(
     const T* __restrict__ logits, long long ld, SelectArgs a, int S, int slice) {
   rnet_dev::pdl_trigger();
   __shared__ Lists lists;
-  __shared__ Selection sel;
+  extern __shared__ uint4 cluster_buf[];
+  Selection& sel = *reinterpret_cast<Selection*>(cluster_buf);
   const int tid = threadIdx.x, rank = blockIdx.y, C = gridDim.y;
   const size_t m0 = (size_t)blockIdx.x * a.W;
   // the first CTA's shared memory may be written once it runs
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   bool waited = C == 1;
+  uint32_t parity;
+  select_setup(sel, parity);
   for (int u = rank; u < a.W * S; u += C) {
     const int beam = u / S, begin = (u % S) * slice, end = min(begin + slice, a.V);
     float m = 0.f;
     double s = 0.0;
     int n = 0;
     if (!(a.finished_in && a.finished_in[m0 + beam]))
-      n = cta_select(sel, logits + (m0 + beam) * ld, min(begin, a.V), end, a.W, LOG2E, m, s);
+      n = cta_select(sel, logits + (m0 + beam) * ld, min(begin, a.V), end, a.W, LOG2E, m, s,
+                     parity, a.err);
     if (!waited) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     waited = true;
     if (tid < n) store_u64(in_first_cta(&lists.key[u][tid]), sel.key[tid]);
@@ -174,23 +179,32 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
   constexpr int N = Words<T>::N;
   const int block = 32 * a.W;
   const size_t smem = (size_t)a.W * WARP_CAP * sizeof(uint64_t);
-  if (a.V <= 256) {
-    beam_select_warps_kernel<T, 8 / N><<<batch, block, smem, s>>>(z, ld, a);
+  if (a.V <= 256 && a.W <= 8) {
+    beam_select_warps_kernel<T, 8 / N, 8><<<batch, block, smem, s>>>(z, ld, a);
     return cudaGetLastError();
   }
-  if (a.V <= 1024) {
-    beam_select_warps_kernel<T, 32 / N><<<batch, block, smem, s>>>(z, ld, a);
+  if (a.V <= 256) {
+    beam_select_warps_kernel<T, 8 / N, 32><<<batch, block, smem, s>>>(z, ld, a);
+    return cudaGetLastError();
+  }
+  if (a.V <= 1024 && a.W <= 8) {  // more beams leave a thread too few registers for the row
+    beam_select_warps_kernel<T, 32 / N, 8><<<batch, block, smem, s>>>(z, ld, a);
     return cudaGetLastError();
   }
   // slices of a row where the rows alone leave SMs idle, one pass or more each
   int S = 1;
   const int pass = SEL_THREADS * SEL_R * N;
   while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * pass < a.V) ++S;
-  const int slice = (((a.V + S - 1) / S) + 1) & ~1;
+  const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
   const int C = a.W * S < 8 ? a.W * S : 8;
+  auto kernel = beam_select_cluster_kernel<T>;
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem((const void*)kernel, sizeof(Selection), ready);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch, C);
   cfg.blockDim = dim3(SEL_THREADS);
+  cfg.dynamicSmemBytes = sizeof(Selection);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -198,7 +212,7 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
   at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, beam_select_cluster_kernel<T>, z, ld, a, S, slice);
+  return cudaLaunchKernelEx(&cfg, kernel, z, ld, a, S, slice);
 }
 
 // ---------------------------------------------------------------- states
@@ -295,9 +309,10 @@ cudaError_t reorder_as(const char* src, char* dst, size_t row_bytes, size_t pitc
 
 cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float* scores_in,
                         const int* finished_in, int eos, float* scores, int* tokens, int* parents,
-                        int* finished, int batch, int beams, int V, cudaStream_t s) {
+                        int* finished, int batch, int beams, int V, unsigned* err, cudaStream_t s) {
   if (batch <= 0) return cudaSuccess;
-  const SelectArgs a{scores_in, finished_in, eos, scores, tokens, parents, finished, beams, V};
+  const SelectArgs a{scores_in, finished_in, eos, scores, tokens, parents, finished, beams, V,
+                     err};
   const cudaError_t e = bf16 ? select_launch((const __nv_bfloat16*)logits, ld, a, batch, s)
                              : select_launch((const float*)logits, ld, a, batch, s);
   return e != cudaSuccess ? e : launched();

@@ -55,7 +55,7 @@ int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float 
            aligned(lse, 4),
        "topk_logits_forward: a pointer is not aligned to its element size");
   CK(rnet_k::topk_logits(logits, dtype == RNET_DTYPE_BF16, ld, temperature, top_logits, top_idx,
-                         lse, rows, vocab, top_k, (cudaStream_t)stream));
+                         lse, rows, vocab, top_k, ew(), (cudaStream_t)stream));
   return RNET_OK;
 }
 
@@ -113,7 +113,8 @@ int rnet_beam_select(const void* logits, int dtype, long long ld, const float* s
            aligned(scores, 4) && aligned(tokens, 4) && aligned(parents, 4) && aligned(finished, 4),
        "beam_select: a pointer is not aligned to its element size");
   CK(rnet_k::beam_select(logits, dtype == RNET_DTYPE_BF16, ld, scores_in, finished_in, eos, scores,
-                         tokens, parents, finished, batch, beams, vocab, (cudaStream_t)stream));
+                         tokens, parents, finished, batch, beams, vocab, ew(),
+                         (cudaStream_t)stream));
   return RNET_OK;
 }
 

@@ -163,7 +163,8 @@ cudaError_t sample_rows(const float* logits, int M, int V, float temperature, fl
 // the row's logits above -inf get -inf / -1. lse (optional) [rows]:
 // log sum exp(logit / tau).
 cudaError_t topk_logits(const void* logits, bool bf16, long long ld, float tau, float* top,
-                        int* idx, float* lse, int rows, int V, int K, cudaStream_t s);
+                        int* idx, float* lse, int rows, int V, int K, unsigned* err,
+                        cudaStream_t s);
 // Loss of each row against a teacher's record, and the gradient:
 //   row_loss = w (soft tau^2 sum_k p_k (log p_k - log softmax(z/tau)[i_k]) + hard CE(z, target))
 //   dl = scale * d row_loss / dz            (dl may be null, or the logits themselves)
@@ -181,7 +182,7 @@ cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int*
 // own score only. Outputs may be the inputs of the same name.
 cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float* scores_in,
                         const int* finished_in, int eos, float* scores, int* tokens, int* parents,
-                        int* finished, int batch, int beams, int V, cudaStream_t s);
+                        int* finished, int batch, int beams, int V, unsigned* err, cudaStream_t s);
 // dst row j of each group of `beams` rows = src row parents[j]; dst may be src.
 cudaError_t beam_reorder(const void* src, void* dst, size_t row_bytes, size_t pitch, size_t outer,
                          size_t outer_pitch, const int* parents, int batch, int beams,

@@ -5,12 +5,25 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
 #include "common.cuh"
 
 namespace rnet_logits {
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once
+// per device: `ready` is the kernel's own record of devices.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (ready.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -1,7 +1,5 @@
 // Records of a row's largest logits, and the distillation loss against such
 // records with its gradient.
-#include <atomic>
-
 #include "common.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
@@ -22,6 +20,7 @@ struct TopkArgs {
   int* idx;
   float* lse;
   int V, K;
+  unsigned* err;
 };
 
 __device__ __forceinline__ void write_place(const TopkArgs& a, size_t row, int k, bool in,
@@ -47,11 +46,10 @@ __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __r
   uint32_t w[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) w[j] = load_word(z, lane + 32 * j, a.V, even);
-  float m;
-  double s;
+  float m, s;
   const int n = warp_select<T, R>(w, a.K, a.c, keys[warp], m, s);
   for (int k = lane; k < a.K; k += 32) write_place(a, row, k, k < n, keys[warp][k]);
-  if (lane == 0 && a.lse) a.lse[row] = (float)log_sum(m, s, a.inv_tau);
+  if (lane == 0 && a.lse) a.lse[row] = log_sum(m, s, a.inv_tau);
 }
 
 // Longer rows: a CTA per row.
@@ -63,10 +61,12 @@ __global__ void __launch_bounds__(SEL_THREADS) topk_cta_kernel(const T* __restri
   const size_t row = blockIdx.x;
   float m;
   double s;
-  const int n = cta_select(sel, logits + row * ld, 0, a.V, a.K, a.c, m, s);
+  uint32_t parity;
+  select_setup(sel, parity);
+  const int n = cta_select(sel, logits + row * ld, 0, a.V, a.K, a.c, m, s, parity, a.err);
   if (threadIdx.x < a.K)
     write_place(a, row, threadIdx.x, threadIdx.x < n, sel.key[threadIdx.x]);
-  if (threadIdx.x == 0 && a.lse) a.lse[row] = (float)log_sum(m, s, a.inv_tau);
+  if (threadIdx.x == 0 && a.lse) a.lse[row] = log_sum(m, (float)s, a.inv_tau);
 }
 
 template <class T>
@@ -623,16 +623,9 @@ cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const Di
   if (C > CLUSTER) C = CLUSTER;
   const int per = (pieces + C - 1) / C;
   if (per > CHUNK * CHUNKS) return cudaErrorInvalidValue;
-  static std::atomic<uint64_t> ready{0};  // devices whose limit is raised
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem((const void*)kernel, 16 * CHUNK * CHUNKS, ready);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             16 * CHUNK * CHUNKS);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows, C);
   cfg.blockDim = dim3(LONG);
@@ -713,9 +706,10 @@ cudaError_t sum_rows(const float* x, int n, float* out, cudaStream_t s) {
 }  // namespace
 
 cudaError_t topk_logits(const void* logits, bool bf16, long long ld, float tau, float* top,
-                        int* idx, float* lse, int rows, int V, int K, cudaStream_t s) {
+                        int* idx, float* lse, int rows, int V, int K, unsigned* err,
+                        cudaStream_t s) {
   if (rows <= 0) return cudaSuccess;
-  const TopkArgs a{LOG2E / tau, 1.0f / tau, top, idx, lse, V, K};
+  const TopkArgs a{LOG2E / tau, 1.0f / tau, top, idx, lse, V, K, err};
   if (bf16) topk_launch((const __nv_bfloat16*)logits, ld, a, rows, s);
   else topk_launch((const float*)logits, ld, a, rows, s);
   return launched();

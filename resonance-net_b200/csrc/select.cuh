@@ -1,13 +1,17 @@
 // The K largest logits of a row with its sum of exponentials, in one pass over
-// the row: by a warp (short rows, held in registers) or by a CTA (streamed).
+// the row: by a warp (short rows, held in registers) or by a CTA (streamed
+// through shared memory).
 //
 // Both work from a bound T that at least K logits are known to reach: with the
 // largest logit of every thread at hand, the r-th largest of a warp's 32 is
 // reached by r logits of that warp. The few logits that reach T are kept as
-// distinct 64-bit keys (value, then lower index) in shared memory and ranked by
-// counting, so the result does not depend on the order in which they came. Where
-// more reach T than there is room for (ties, sorted rows), the exact K-th key is
-// found bit by bit and becomes the bound.
+// distinct 64-bit keys (value, then lower index) and ranked by counting, so the
+// result does not depend on the order in which they came. Where more reach T than
+// there is room for (ties, sorted rows), the exact K-th key is found bit by bit
+// and becomes the bound.
+//
+// NaN and +inf are not looked for: either makes the sum of exponentials NaN, and
+// only then the row is gone through again with every value made finite.
 //
 // Element e of a row goes to the same thread whatever the row's alignment: equal
 // rows give the same bits, so that equal candidates of a beam search tie.
@@ -22,51 +26,57 @@ struct Words {
   static constexpr int N = 4 / sizeof(T);
 };
 
-// Word w (elements N w, N w + 1) of the row z of elements below end; -inf beyond.
-// NaN reads as -inf.
+// Word w (elements N w, N w + 1) of a row z of `end` elements, -inf beyond.
 __device__ __forceinline__ uint32_t load_word(const float* z, int w, int end, bool) {
-  return __float_as_uint(fmaxf(w < end ? z[w] : -INFINITY, -INFINITY));
+  return w < end ? __float_as_uint(z[w]) : 0xFF800000u;
 }
 __device__ __forceinline__ uint32_t load_word(const __nv_bfloat16* z, int w, int end, bool even) {
   const int e = 2 * w;
-  uint32_t u = 0xFF80FF80u;
-  if (even && e + 1 < end) {  // the row starts on a 4-byte boundary
-    u = *reinterpret_cast<const uint32_t*>(z + e);
-  } else {
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(z);
-    if (e < end) u = 0xFF800000u | p[e];
-    if (e + 1 < end) u = (u & 0xFFFFu) | (uint32_t)p[e + 1] << 16;
-  }
-  const uint32_t none = 0xFF80FF80u;
-  const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&u),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&none));
-  return *reinterpret_cast<const uint32_t*>(&h);
+  if (even && e + 1 < end)  // the row starts on a 4-byte boundary
+    return *reinterpret_cast<const uint32_t*>(z + e);
+  const unsigned short* p = reinterpret_cast<const unsigned short*>(z);
+  const uint32_t lo = e < end ? p[e] : 0xFF80u, hi = e + 1 < end ? p[e + 1] : 0xFF80u;
+  return lo | hi << 16;
 }
 template <class T>
 __device__ __forceinline__ bool even_start(const T* z) {
   return ((uintptr_t)z & 3) == 0;
 }
-// Value i of a word; +inf as the largest number.
-template <class T>
+// Value i of a word; CLEAN: NaN as -inf, +inf as the largest number.
+template <class T, bool CLEAN>
 __device__ __forceinline__ float word_value(uint32_t w, int i) {
-  if constexpr (sizeof(T) == 4) return fminf(__uint_as_float(w), FLT_MAX);
-  else return fminf(__uint_as_float(i ? w & 0xFFFF0000u : w << 16), FLT_MAX);
+  float x;
+  if constexpr (sizeof(T) == 4) x = __uint_as_float(w);
+  else x = __uint_as_float(i ? w & 0xFFFF0000u : w << 16);
+  return CLEAN ? fminf(fmaxf(x, -INFINITY), FLT_MAX) : x;
 }
 // The largest value of R words.
-template <class T, int R>
+template <class T, int R, bool CLEAN>
 __device__ __forceinline__ float words_max(const uint32_t* w) {
+  float m;
   if constexpr (sizeof(T) == 4) {
-    float m = __uint_as_float(w[0]);
+    m = fmaxf(__uint_as_float(w[0]), -INFINITY);
 #pragma unroll
     for (int j = 1; j < R; ++j) m = fmaxf(m, __uint_as_float(w[j]));
-    return fminf(m, FLT_MAX);
   } else {
     auto h = [&](int j) { return *reinterpret_cast<const __nv_bfloat162*>(&w[j]); };
-    __nv_bfloat162 m = h(0);
+    __nv_bfloat162 a = h(0);
 #pragma unroll
-    for (int j = 1; j < R; ++j) m = __hmax2(m, h(j));
-    return fminf(fmaxf(__low2float(m), __high2float(m)), FLT_MAX);
+    for (int j = 1; j < R; ++j) a = __hmax2(a, h(j));
+    m = fmaxf(fmaxf(__low2float(a), __high2float(a)), -INFINITY);
   }
+  return CLEAN ? fminf(m, FLT_MAX) : m;
+}
+// Sum of 2^((x - m) c) over R words. m + 0 > -inf.
+template <class T, int R, bool CLEAN>
+__device__ __forceinline__ float words_sum(const uint32_t* w, float m, float c) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < R; ++j)
+#pragma unroll
+    for (int i = 0; i < Words<T>::N; ++i)
+      s += exp2_fast((word_value<T, CLEAN>(w[j], i) - m) * c);
+  return s;
 }
 
 // The r-th largest (r = 1..32) of a warp's 32 values.
@@ -84,79 +94,90 @@ __device__ __forceinline__ float warp_nth(float v, int r) {
   return __shfl_sync(~0u, v, r - 1);
 }
 
-__device__ __forceinline__ double warp_sum_d(double v) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
 }
 
-// log of the sum of exponentials at c = log2(e) / tau from the largest logit m
-// and the sum s of 2^((x - m) c); -inf for a row without a logit above -inf.
-__device__ __forceinline__ double log_sum(float m, double s, float inv_tau) {
-  return s > 0.0 ? (double)m * (double)inv_tau + log(s) : -(double)INFINITY;
+// log of the sum of exponentials at tau from the largest logit m and the sum s of
+// 2^((x - m) log2(e) / tau); -inf for a row without a logit above -inf.
+__device__ __forceinline__ float log_sum(float m, float s, float inv_tau) {
+  return s > 0.f ? m * inv_tau + LN2 * log2_fast(s) : -INFINITY;
+}
+__device__ __forceinline__ double log_sum(float m, double s) {
+  return s > 0.0 ? (double)m + log(s) : -(double)INFINITY;
 }
 
 // ---------------------------------------------------------------- a warp
 constexpr int WARP_CAP = 128;  // keys kept at most
 
-// The K <= 64 largest of the words of a row of V elements, word lane + 32 j in
-// w[j]. key[0 .. return value) are sorted; key has WARP_CAP places. m and s as
-// for log_sum.
-template <class T, int R>
-__device__ __forceinline__ int warp_select(const uint32_t* w, int K, float c, uint64_t* key,
-                                           float& m, double& s) {
+// The K <= 64 largest of the words of a row, word lane + 32 j in w[j]. key[0 ..
+// return value) are sorted; key has WARP_CAP places. m is the row's largest
+// logit, s the sum as Sum.
+template <class T, int R, bool CLEAN, class Sum>
+__device__ __forceinline__ int warp_select_as(const uint32_t* w, int K, float c, uint64_t* key,
+                                              float& m, Sum& s) {
   constexpr int N = Words<T>::N;
   const int lane = threadIdx.x & 31;
   auto each = [&](auto f) {
 #pragma unroll
     for (int j = 0; j < R; ++j)
 #pragma unroll
-      for (int i = 0; i < N; ++i) f(word_value<T>(w[j], i), (lane + 32 * j) * N + i);
+      for (int i = 0; i < N; ++i) f(word_value<T, CLEAN>(w[j], i), (lane + 32 * j) * N + i);
   };
-  const float mine = words_max<T, R>(w);
+  const float mine = words_max<T, R, CLEAN>(w);
   m = fmaxf(warp_max(mine), -FLT_MAX);
-  float sum = 0.f;
-  each([&](float x, int) { sum += exp2_fast((x - m) * c); });
-  s = warp_sum_d(sum);
+  s = warp_sum((Sum)words_sum<T, R, CLEAN>(w, m, c));
+  if (!CLEAN && s != s) return 0;
   // K logits reach T: from K lanes, or two each from K / 2 lanes
   float T_;
   if (K <= 32 || R == 1) {
     T_ = K <= 32 ? warp_nth(mine, K) : -INFINITY;
   } else {
     constexpr int H = (R + 1) / 2;
-    T_ = warp_nth(fminf(words_max<T, H>(w), words_max<T, R - H ? R - H : 1>(w + H % R)),
+    T_ = warp_nth(fminf(words_max<T, H, CLEAN>(w),
+                        words_max<T, R - H ? R - H : 1, CLEAN>(w + H % R)),
                   (K + 1) / 2);
   }
-  int count = 0;
-  each([&](float x, int) { count += x >= T_ && x > -INFINITY; });
-  uint32_t last = ~0u;  // of the logits equal to T, those up to this index
-  if (__reduce_add_sync(~0u, count) > WARP_CAP) {
+  T_ = fmaxf(T_, -FLT_MAX);  // -inf is no candidate
+  int mine_in = 0;
+  each([&](float x, int) { mine_in += x >= T_; });
+  int at = mine_in;  // keys of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, at, o);
+    if (lane >= o) at += v;
+  }
+  int n = __shfl_sync(~0u, at, 31);
+  at -= mine_in;
+  if (n <= WARP_CAP) {
+    each([&](float x, int e) {
+      if (x >= T_) key[at++] = make_key(x + 0.0f, e);
+    });
+  } else {
     // the exact K-th largest value, bit by bit, and how many of its equals count
     auto reach = [&](auto f) {
-      int n = 0;
-      each([&](float x, int e) { n += x > -INFINITY && f(order(x + 0.0f), (uint32_t)e); });
-      return __reduce_add_sync(~0u, n);
+      int k = 0;
+      each([&](float x, int e) { k += x > -INFINITY && f(order(x + 0.0f), (uint32_t)e); });
+      return __reduce_add_sync(~0u, k);
     };
-    uint32_t o = 0;
+    uint32_t o = 0, last = 0;
     for (uint32_t b = 1u << 31; b; b >>= 1)
       if (reach([&](uint32_t x, uint32_t) { return x >= (o | b); }) >= K) o |= b;
     const int above = reach([&](uint32_t x, uint32_t) { return x > o; });
-    last = 0;
     for (uint32_t b = 1u << 10; b; b >>= 1)
       if (reach([&](uint32_t x, uint32_t e) { return x == o && e < (last | b); }) < K - above)
         last |= b;
-    T_ = unorder(o);
-  }
-  // keys of the logits that reach the bound
-  int n = 0;
-  each([&](float x, int e) {
-    const bool in = x > -INFINITY && (x > T_ || (x == T_ && (uint32_t)e <= last));
-    const uint32_t mask = __ballot_sync(~0u, in);
-    if (mask) {
+    n = 0;
+    each([&](float x, int e) {
+      const uint32_t v = order(x + 0.0f);
+      const bool in = x > -INFINITY && (v > o || (v == o && (uint32_t)e <= last));
+      const uint32_t mask = __ballot_sync(~0u, in);
       if (in) key[n + __popc(mask & ((1u << lane) - 1))] = make_key(x + 0.0f, e);
       n += __popc(mask);
-    }
-  });
+    });
+  }
   __syncwarp();
   // each key's place is the number of larger ones
   uint64_t own[WARP_CAP / 32];
@@ -176,23 +197,47 @@ __device__ __forceinline__ int warp_select(const uint32_t* w, int K, float c, ui
   __syncwarp();
   return min(n, K);
 }
+template <class T, int R, class Sum>
+__device__ __forceinline__ int warp_select(const uint32_t* w, int K, float c, uint64_t* key,
+                                           float& m, Sum& s) {
+  const int n = warp_select_as<T, R, false>(w, K, c, key, m, s);
+  return s == s ? n : warp_select_as<T, R, true>(w, K, c, key, m, s);
+}
 
 // ---------------------------------------------------------------- a CTA
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
-constexpr int SEL_R = 16;     // words of a thread at a time
-constexpr int SEL_CAP = 1024; // keys kept at most
+constexpr int SEL_R = 16;             // words of a thread in one chunk
+constexpr int SEL_GROUP = 4;          // words that are kept together
+constexpr int SEL_STAGES = 2;         // chunks in shared memory
+constexpr int SEL_CHUNK = SEL_THREADS * SEL_R;  // words
+constexpr int SEL_QUEUE = 256;        // groups kept at most
+constexpr int SEL_CAP = 512;          // keys kept at most
 
-struct Selection {
+struct alignas(16) Selection {
+  uint32_t ring[SEL_STAGES][SEL_CHUNK + 4];
+  uint32_t group[SEL_GROUP][SEL_QUEUE];
+  int group_word[SEL_QUEUE];  // the group's first word
   uint64_t key[SEL_CAP];
-  float bound[SEL_WARPS], m[SEL_WARPS];
   double s[SEL_WARPS];
-  int count;
+  float bound[SEL_WARPS], m[SEL_WARPS];
+  uint64_t bar[SEL_STAGES];
+  int keys, groups, abort[2];
 };
 
-// Leaves the K largest of the n <= SEL_CAP keys that `keep` accepts, in any
-// order, and returns a bound that exactly they reach (0 if there are no more
-// than K). All threads.
+// Once per CTA, before the first selection; parity belongs to the barriers.
+__device__ __forceinline__ void select_setup(Selection& sel, uint32_t& parity) {
+  parity = 0;
+  if (threadIdx.x == 0) {
+    sel.abort[0] = sel.abort[1] = 0;
+    for (int i = 0; i < SEL_STAGES; ++i) rnet_dev::mbar_init(&sel.bar[i], 1);
+    rnet_dev::fence_barrier_init();
+  }
+}
+
+// Leaves the K largest of the n <= SEL_CAP keys, or those of them that `keep`
+// accepts, in any order, and returns a bound that exactly K of all n reach (0 if
+// there are no more than K). All threads, which have read n before.
 template <class Keep>
 __device__ __forceinline__ uint64_t shrink(Selection& sel, int n, int K, Keep keep) {
   constexpr int J = SEL_CAP / SEL_THREADS;
@@ -214,94 +259,199 @@ __device__ __forceinline__ uint64_t shrink(Selection& sel, int n, int K, Keep ke
       if (reach == K) break;
     }
   __syncthreads();
-  if (threadIdx.x == 0) sel.count = 0;
+  if (threadIdx.x == 0) sel.keys = 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < J; ++j)
-    if (k[j] && k[j] >= t && keep(k[j])) sel.key[atomicAdd(&sel.count, 1)] = k[j];
+    if (k[j] && k[j] >= t && keep(k[j])) sel.key[atomicAdd(&sel.keys, 1)] = k[j];
   __syncthreads();
   return t;
 }
 
-// The K <= 64 largest of the elements [begin, end) of the row z (begin even).
-// sel.key[0 .. return value) are sorted. m and s as for log_sum. All
-// SEL_THREADS threads.
-template <class T>
-__device__ __forceinline__ int cta_select(Selection& sel, const T* z, int begin, int end, int K,
-                                          float c, float& m, double& s) {
-  constexpr int N = Words<T>::N, STEP = SEL_THREADS * SEL_R;  // words a pass
+// Turns the n queued groups into keys that reach the bound. All threads, which
+// have read n before. Where they are more than there is room for, the bound is
+// raised to the K-th of those at hand and the groups are gone through again; the
+// keys of earlier groups (elements before `first`) stay.
+template <class T, bool CLEAN>
+__device__ __forceinline__ void drain(Selection& sel, int n, int K, int first, uint64_t& bound) {
+  constexpr int N = Words<T>::N;
+  for (bool again = true; again;) {
+    for (int i = threadIdx.x; i < n; i += SEL_THREADS) {
+      const int word = sel.group_word[i];
+#pragma unroll
+      for (int j = 0; j < SEL_GROUP; ++j)
+#pragma unroll
+        for (int h = 0; h < N; ++h) {
+          const float x = word_value<T, CLEAN>(sel.group[j][i], h);
+          if (!(x > -INFINITY)) continue;
+          const uint64_t k = make_key(x + 0.0f, (word + j * SEL_THREADS) * N + h);
+          if (k < bound) continue;
+          const int at = atomicAdd(&sel.keys, 1);
+          if (at < SEL_CAP) sel.key[at] = k;
+        }
+    }
+    __syncthreads();
+    const int got = sel.keys;
+    __syncthreads();
+    again = got > SEL_CAP;
+    if (again) {
+      const uint64_t t = shrink(sel, SEL_CAP, K, [&](uint64_t k) {
+        return key_index(k) < first;
+      });
+      bound = t > bound ? t : bound;
+    }
+  }
+}
+
+// The K <= 64 largest of the elements [begin, end) of the row z (begin on a
+// 16-byte place of the row, and a multiple of 2). sel.key[0 .. return value) are
+// sorted. m is the slice's largest logit, s the sum. All SEL_THREADS threads; sel
+// is set up and not in use.
+template <class T, bool CLEAN>
+__device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int begin, int end, int K,
+                                             float c, float& m, double& s, uint32_t& parity,
+                                             unsigned* err) {
+  constexpr int N = Words<T>::N;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool even = even_start(z);
-  if (tid == 0) sel.count = 0;
-  uint64_t bound = 0;
-  float lowest = -INFINITY;  // its value
-  float sum = 0.f;
-  m = -FLT_MAX;
-  uint32_t w[SEL_R];
-  auto load = [&](int w0) {
-#pragma unroll
-    for (int j = 0; j < SEL_R; ++j)
-      w[j] = load_word(z, w0 + j * SEL_THREADS + tid, end, even);
+  const int total = begin < end ? (end - begin + N - 1) / N : 0;  // words
+  const int chunks = (total + SEL_CHUNK - 1) / SEL_CHUNK;
+  const T* zb = z + begin;
+  const uint32_t skew = (uint32_t)((uintptr_t)zb & 15);  // of every chunk's first byte
+  // A chunk comes through shared memory if the 16-byte pieces that cover it lie
+  // inside the slice; the first one of an unaligned row and the last do not.
+  auto staged = [&](int i) {
+    return (i > 0 || skew == 0) && (i + 1) * SEL_CHUNK * N + (skew ? 16 / (int)sizeof(T) : 0) <=
+                                       end - begin;
   };
-  const int w1 = begin < end ? (end + N - 1) / N : 0;
-  for (int w0 = begin / N; w0 < w1; w0 += STEP) {
-    load(w0);
-    const float mine = words_max<T, SEL_R>(w), mx = fmaxf(m, mine);
-    sum *= exp2_fast((m - mx) * c);
+  auto fetch = [&](int i) {  // one thread
+    const uint32_t bytes = SEL_CHUNK * 4 + (skew ? 16 : 0);
+    uint64_t* bar = &sel.bar[i % SEL_STAGES];
+    rnet_dev::mbar_arrive_expect_tx(bar, bytes);
+    bulk_load(sel.ring[i % SEL_STAGES],
+              reinterpret_cast<const char*>(zb + (size_t)i * SEL_CHUNK * N) - skew, bytes, bar);
+  };
+  if (tid == 0) {
+    sel.keys = sel.groups = 0;
+    for (int i = 0; i < SEL_STAGES && i < chunks; ++i)
+      if (staged(i)) fetch(i);
+  }
+  __syncthreads();
+  uint64_t bound = 0;
+  float lowest = -FLT_MAX;  // its value
+  float sum = 0.f;
+  int epoch = begin;        // the queue's elements lie behind this one
+  m = -FLT_MAX;
+  for (int i = 0; i < chunks; ++i) {
+    const int w0 = begin / N + i * SEL_CHUNK;  // the row's first word of the chunk
+    uint32_t w[SEL_R];
+    if (staged(i)) {
+      const int b = i % SEL_STAGES;
+      // a copy that does not come is reported and given the same time once more:
+      // none may land in memory that the CTA has left
+      if (!rnet_dev::mbar_wait(&sel.bar[b], parity >> b & 1, err, &sel.abort[0]))
+        rnet_dev::mbar_wait(&sel.bar[b], parity >> b & 1, err, &sel.abort[1]);
+      parity ^= 1u << b;
+      const char* p = reinterpret_cast<const char*>(sel.ring[b]) + skew + 4 * tid;
+      if (even) {
+#pragma unroll
+        for (int j = 0; j < SEL_R; ++j)
+          w[j] = *reinterpret_cast<const uint32_t*>(p + 4 * SEL_THREADS * j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < SEL_R; ++j) {
+          const unsigned short* q =
+              reinterpret_cast<const unsigned short*>(p + 4 * SEL_THREADS * j);
+          w[j] = q[0] | (uint32_t)q[1] << 16;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < SEL_R; ++j)
+        w[j] = load_word(z, w0 + j * SEL_THREADS + tid, end, even);
+    }
+    float top[SEL_R / SEL_GROUP];
+    float mine = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < SEL_R / SEL_GROUP; ++g) {
+      top[g] = words_max<T, SEL_GROUP, CLEAN>(w + g * SEL_GROUP);
+      mine = fmaxf(mine, top[g]);
+    }
+    const float mx = fmaxf(m, mine);
+    sum = sum * exp2_fast((m - mx) * c) + words_sum<T, SEL_R, CLEAN>(w, mx, c);
     m = mx;
-#pragma unroll
-    for (int j = 0; j < SEL_R; ++j)
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum += exp2_fast((word_value<T>(w[j], i) - m) * c);
-    if (w0 == begin / N) {
+    if (i == 0) {
       // K logits reach the least of the warps' r-th largest thread maxima
       const float v = warp_nth(mine, (K + SEL_WARPS - 1) / SEL_WARPS);
       if (lane == 0) sel.bound[warp] = v;
       __syncthreads();
       lowest = sel.bound[0];
 #pragma unroll
-      for (int i = 1; i < SEL_WARPS; ++i) lowest = fminf(lowest, sel.bound[i]);
+      for (int j = 1; j < SEL_WARPS; ++j) lowest = fminf(lowest, sel.bound[j]);
+      lowest = fmaxf(lowest, -FLT_MAX);
       bound = (uint64_t)order(lowest + 0.0f) << 32;
     }
+    // a group whose largest logit equals the bound's value: by its keys
+    auto reaches = [&](int g) {
+      bool in = false;
+#pragma unroll
+      for (int j = 0; j < SEL_GROUP; ++j)
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+          in |= make_key(word_value<T, CLEAN>(w[g * SEL_GROUP + j], h) + 0.0f,
+                         (w0 + (g * SEL_GROUP + j) * SEL_THREADS + tid) * N + h) >= bound;
+      return in;
+    };
     for (bool again = true; again;) {
       bool full = false;
-      if (mine >= lowest && mine > -INFINITY) {
 #pragma unroll
-        for (int j = 0; j < SEL_R; ++j)
+      for (int g = 0; g < SEL_R / SEL_GROUP; ++g)
+        if (top[g] > lowest || (top[g] == lowest && reaches(g))) {
+          const int at = atomicAdd(&sel.groups, 1);
+          full |= at >= SEL_QUEUE / 2;
+          if (at < SEL_QUEUE) {
+            sel.group_word[at] = w0 + g * SEL_GROUP * SEL_THREADS + tid;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float x = word_value<T>(w[j], i);
-            if (x < lowest || x == -INFINITY) continue;
-            const uint64_t k = make_key(x + 0.0f, (w0 + j * SEL_THREADS + tid) * N + i);
-            if (k < bound) continue;
-            const int at = atomicAdd(&sel.count, 1);
-            if (at < SEL_CAP) sel.key[at] = k;
-            full |= at >= SEL_CAP / 2;
+            for (int j = 0; j < SEL_GROUP; ++j) sel.group[j][at] = w[g * SEL_GROUP + j];
           }
-      }
+        }
       again = false;
       if (__syncthreads_or(full)) {
-        const int n = sel.count;
+        const int n = sel.groups;
         __syncthreads();
-        // beyond the room: this pass's keys are dropped and come again
-        again = n > SEL_CAP;
-        const uint32_t first = w0 * N;
-        bound = shrink(sel, min(n, SEL_CAP), K, [&](uint64_t k) {
-          return !again || (uint32_t)key_index(k) < first;
+        again = n > SEL_QUEUE;  // then this chunk's groups come again
+        drain<T, CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound);
+        const int got = sel.keys, here = w0 * N;
+        __syncthreads();
+        const uint64_t t = shrink(sel, got, K, [&](uint64_t k) {
+          return !again || key_index(k) < here;
         });
-        if (bound) lowest = key_value(bound);
+        bound = t > bound ? t : bound;
+        lowest = fmaxf(lowest, key_value(bound));
+        if (tid == 0) sel.groups = 0;
+        epoch = again ? here : here + SEL_CHUNK * N;
+        __syncthreads();
       }
     }
+    // the chunk's place is free
+    if (tid == 0 && i + SEL_STAGES < chunks && staged(i + SEL_STAGES)) fetch(i + SEL_STAGES);
   }
   __syncthreads();
-  int n = sel.count;
+  {
+    const int n = sel.groups;
+    __syncthreads();
+    drain<T, CLEAN>(sel, n, K, epoch, bound);
+  }
+  int n = sel.keys;
+  __syncthreads();
   if (n > SEL_THREADS) {
     shrink(sel, n, K, [](uint64_t) { return true; });
-    n = sel.count;
+    n = sel.keys;
   }
   const uint64_t own = tid < n ? sel.key[tid] : 0;
   int place = 0;
-  for (int k = 0; k < n; ++k) place += sel.key[k] > own;
+  if (tid < ((n + 31) & ~31))
+    for (int k = 0; k < n; ++k) place += sel.key[k] > own;
   const float mw = warp_max(m);
   if (lane == 0) sel.m[warp] = mw;
   __syncthreads();
@@ -310,13 +460,24 @@ __device__ __forceinline__ int cta_select(Selection& sel, const T* z, int begin,
   m = sel.m[0];
 #pragma unroll
   for (int i = 1; i < SEL_WARPS; ++i) m = fmaxf(m, sel.m[i]);
-  const double part = warp_sum_d((double)(sum * exp2_fast((mine - m) * c)));
+  const double part = warp_sum((double)(sum * exp2_fast((mine - m) * c)));
   if (lane == 0) sel.s[warp] = part;
   __syncthreads();
   s = 0.0;
 #pragma unroll
   for (int i = 0; i < SEL_WARPS; ++i) s += sel.s[i];
   return min(n, K);
+}
+template <class T>
+__device__ __forceinline__ int cta_select(Selection& sel, const T* z, int begin, int end, int K,
+                                          float c, float& m, double& s, uint32_t& parity,
+                                          unsigned* err) {
+  int n = cta_select_as<T, false>(sel, z, begin, end, K, c, m, s, parity, err);
+  if (s != s) {
+    __syncthreads();
+    n = cta_select_as<T, true>(sel, z, begin, end, K, c, m, s, parity, err);
+  }
+  return n;
 }
 
 }  // namespace rnet_logits
