@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __r
 
 // Longer rows: a CTA per row.
 template <class T>
-__global__ void __launch_bounds__(SEL_THREADS) topk_cta_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(SEL_THREADS, 4) topk_cta_kernel(const T* __restrict__ logits,
                                                                long long ld, TopkArgs a) {
   rnet_dev::pdl_trigger();
   __shared__ Selection sel;

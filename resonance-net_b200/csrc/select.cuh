@@ -211,7 +211,7 @@ constexpr int SEL_R = 16;             // words of a thread in one chunk
 constexpr int SEL_GROUP = 4;          // words that are kept together
 constexpr int SEL_STAGES = 2;         // chunks in shared memory
 constexpr int SEL_CHUNK = SEL_THREADS * SEL_R;  // words
-constexpr int SEL_QUEUE = 256;        // groups kept at most
+constexpr int SEL_QUEUE = 512;        // groups kept at most
 constexpr int SEL_CAP = 512;          // keys kept at most
 
 struct alignas(16) Selection {
@@ -220,7 +220,7 @@ struct alignas(16) Selection {
   int group_word[SEL_QUEUE];  // the group's first word
   uint64_t key[SEL_CAP];
   double s[SEL_WARPS];
-  float bound[SEL_WARPS], m[SEL_WARPS];
+  float bound[2][SEL_WARPS], m[SEL_WARPS];
   uint64_t bar[SEL_STAGES];
   int keys, groups, abort[2];
 };
@@ -339,6 +339,7 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
   __syncthreads();
   uint64_t bound = 0;
   float lowest = -FLT_MAX;  // its value
+  bool exact = false;       // the bound is a key of the row, not a value alone
   float sum = 0.f;
   int epoch = begin;        // the queue's elements lie behind this one
   m = -FLT_MAX;
@@ -380,41 +381,55 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
     const float mx = fmaxf(m, mine);
     sum = sum * exp2_fast((m - mx) * c) + words_sum<T, SEL_R, CLEAN>(w, mx, c);
     m = mx;
-    if (i == 0) {
-      // K logits reach the least of the warps' r-th largest thread maxima
-      const float v = warp_nth(mine, (K + SEL_WARPS - 1) / SEL_WARPS);
-      if (lane == 0) sel.bound[warp] = v;
+    if (i < 4 || (i & 3) == 0) {
+      // K logits reach the least of the warps' r-th largest thread maxima so far
+      const float v = warp_nth(m, (K + SEL_WARPS - 1) / SEL_WARPS);
+      if (lane == 0) sel.bound[i & 1][warp] = v;
       __syncthreads();
-      lowest = sel.bound[0];
+      float least = sel.bound[i & 1][0];
 #pragma unroll
-      for (int j = 1; j < SEL_WARPS; ++j) lowest = fminf(lowest, sel.bound[j]);
-      lowest = fmaxf(lowest, -FLT_MAX);
-      bound = (uint64_t)order(lowest + 0.0f) << 32;
+      for (int j = 1; j < SEL_WARPS; ++j) least = fminf(least, sel.bound[i & 1][j]);
+      const uint64_t t = (uint64_t)order(least + 0.0f) << 32;
+      if (t > bound) {
+        bound = t;
+        lowest = least;
+        exact = false;
+      }
     }
-    // a group whose largest logit equals the bound's value: by its keys
+    // where the bound is a key, a group whose largest logit equals its value
+    // is looked at key by key (the volatile move keeps the compiler from forming all
+    // the keys ahead of time)
     auto reaches = [&](int g) {
       bool in = false;
 #pragma unroll
-      for (int j = 0; j < SEL_GROUP; ++j)
+      for (int j = 0; j < SEL_GROUP; ++j) {
+        uint32_t v;
+        asm volatile("mov.b32 %0, %1;" : "=r"(v) : "r"(w[g * SEL_GROUP + j]));
 #pragma unroll
         for (int h = 0; h < N; ++h)
-          in |= make_key(word_value<T, CLEAN>(w[g * SEL_GROUP + j], h) + 0.0f,
+          in |= make_key(word_value<T, CLEAN>(v, h) + 0.0f,
                          (w0 + (g * SEL_GROUP + j) * SEL_THREADS + tid) * N + h) >= bound;
+      }
       return in;
     };
-    for (bool again = true; again;) {
-      bool full = false;
+    bool full;
+    auto queue = [&](auto wanted) {
 #pragma unroll
       for (int g = 0; g < SEL_R / SEL_GROUP; ++g)
-        if (top[g] > lowest || (top[g] == lowest && reaches(g))) {
+        if (top[g] >= lowest && wanted(g)) {
           const int at = atomicAdd(&sel.groups, 1);
-          full |= at >= SEL_QUEUE / 2;
+          full |= at >= SEL_QUEUE - SEL_QUEUE / 4;
           if (at < SEL_QUEUE) {
             sel.group_word[at] = w0 + g * SEL_GROUP * SEL_THREADS + tid;
 #pragma unroll
             for (int j = 0; j < SEL_GROUP; ++j) sel.group[j][at] = w[g * SEL_GROUP + j];
           }
         }
+    };
+    for (bool again = true; again;) {
+      full = false;
+      if (!exact) queue([](int) { return true; });
+      else queue([&](int g) { return top[g] > lowest || reaches(g); });
       again = false;
       if (__syncthreads_or(full)) {
         const int n = sel.groups;
@@ -427,7 +442,8 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
           return !again || key_index(k) < here;
         });
         bound = t > bound ? t : bound;
-        lowest = fmaxf(lowest, key_value(bound));
+        lowest = key_value(bound);
+        exact = true;
         if (tid == 0) sel.groups = 0;
         epoch = again ? here : here + SEL_CHUNK * N;
         __syncthreads();
