@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(SEL_THREADS) beam_select_cluster_kernel(
   rnet_dev::pdl_trigger();
   __shared__ Lists lists;
   extern __shared__ uint4 cluster_buf[];
-  Selection& sel = *reinterpret_cast<Selection*>(cluster_buf);
+  Selection<T>& sel = *reinterpret_cast<Selection<T>*>(cluster_buf);
   const int tid = threadIdx.x, rank = blockIdx.y, C = gridDim.y;
   const size_t m0 = (size_t)blockIdx.x * a.W;
   // the first CTA's shared memory may be written once it runs
@@ -193,18 +193,17 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
   }
   // slices of a row where the rows alone leave SMs idle, one pass or more each
   int S = 1;
-  const int pass = SEL_THREADS * SEL_R * N;
-  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * pass < a.V) ++S;
+  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * Selection<T>::CHUNK * N < a.V) ++S;
   const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
   const int C = a.W * S < 8 ? a.W * S : 8;
   auto kernel = beam_select_cluster_kernel<T>;
   static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem((const void*)kernel, sizeof(Selection), ready);
+  cudaError_t e = allow_smem((const void*)kernel, sizeof(Selection<T>), ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch, C);
   cfg.blockDim = dim3(SEL_THREADS);
-  cfg.dynamicSmemBytes = sizeof(Selection);
+  cfg.dynamicSmemBytes = sizeof(Selection<T>);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -54,10 +54,11 @@ __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __r
 
 // Longer rows: a CTA per row.
 template <class T>
-__global__ void __launch_bounds__(SEL_THREADS, 4) topk_cta_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(SEL_THREADS, sizeof(T) == 2 ? 4 : 2) topk_cta_kernel(const T* __restrict__ logits,
                                                                long long ld, TopkArgs a) {
   rnet_dev::pdl_trigger();
-  __shared__ Selection sel;
+  extern __shared__ uint4 sel_buf[];
+  Selection<T>& sel = *reinterpret_cast<Selection<T>*>(sel_buf);
   const size_t row = blockIdx.x;
   float m;
   double s;
@@ -70,15 +71,21 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) topk_cta_kernel(const T* __res
 }
 
 template <class T>
-void topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
+cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
   constexpr int N = Words<T>::N;
   const int grid = (rows + TOPK_WARPS - 1) / TOPK_WARPS, block = 32 * TOPK_WARPS;
   if (a.V <= 256)
     topk_warp_kernel<T, 8 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
   else if (a.V <= 1024)
     topk_warp_kernel<T, 32 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
-  else
-    topk_cta_kernel<T><<<rows, SEL_THREADS, 0, s>>>(z, ld, a);
+  else {
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e =
+        allow_smem((const void*)topk_cta_kernel<T>, sizeof(Selection<T>), ready);
+    if (e != cudaSuccess) return e;
+    topk_cta_kernel<T><<<rows, SEL_THREADS, sizeof(Selection<T>), s>>>(z, ld, a);
+  }
+  return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------- distillation
@@ -710,9 +717,9 @@ cudaError_t topk_logits(const void* logits, bool bf16, long long ld, float tau, 
                         cudaStream_t s) {
   if (rows <= 0) return cudaSuccess;
   const TopkArgs a{LOG2E / tau, 1.0f / tau, top, idx, lse, V, K, err};
-  if (bf16) topk_launch((const __nv_bfloat16*)logits, ld, a, rows, s);
-  else topk_launch((const float*)logits, ld, a, rows, s);
-  return launched();
+  const cudaError_t e = bf16 ? topk_launch((const __nv_bfloat16*)logits, ld, a, rows, s)
+                             : topk_launch((const float*)logits, ld, a, rows, s);
+  return e != cudaSuccess ? e : launched();
 }
 
 cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int* t_idx,

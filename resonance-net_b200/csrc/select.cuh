@@ -207,15 +207,17 @@ __device__ __forceinline__ int warp_select(const uint32_t* w, int K, float c, ui
 // ---------------------------------------------------------------- a CTA
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
-constexpr int SEL_R = 16;             // words of a thread in one chunk
 constexpr int SEL_GROUP = 4;          // words that are kept together
 constexpr int SEL_STAGES = 2;         // chunks in shared memory
-constexpr int SEL_CHUNK = SEL_THREADS * SEL_R;  // words
 constexpr int SEL_QUEUE = 512;        // groups kept at most
 constexpr int SEL_CAP = 512;          // keys kept at most
 
+template <class T>
 struct alignas(16) Selection {
-  uint32_t ring[SEL_STAGES][SEL_CHUNK + 4];
+  static constexpr int N = Words<T>::N;
+  static constexpr int R = 32 / N;             // words of a thread in one chunk
+  static constexpr int CHUNK = SEL_THREADS * R;  // words
+  uint32_t ring[SEL_STAGES][CHUNK + 4];
   uint32_t group[SEL_GROUP][SEL_QUEUE];
   int group_word[SEL_QUEUE];  // the group's first word
   uint64_t key[SEL_CAP];
@@ -226,7 +228,8 @@ struct alignas(16) Selection {
 };
 
 // Once per CTA, before the first selection; parity belongs to the barriers.
-__device__ __forceinline__ void select_setup(Selection& sel, uint32_t& parity) {
+template <class T>
+__device__ __forceinline__ void select_setup(Selection<T>& sel, uint32_t& parity) {
   parity = 0;
   if (threadIdx.x == 0) {
     sel.abort[0] = sel.abort[1] = 0;
@@ -238,8 +241,8 @@ __device__ __forceinline__ void select_setup(Selection& sel, uint32_t& parity) {
 // Leaves the K largest of the n <= SEL_CAP keys, or those of them that `keep`
 // accepts, in any order, and returns a bound that exactly K of all n reach (0 if
 // there are no more than K). All threads, which have read n before.
-template <class Keep>
-__device__ __forceinline__ uint64_t shrink(Selection& sel, int n, int K, Keep keep) {
+template <class T, class Keep>
+__device__ __forceinline__ uint64_t shrink(Selection<T>& sel, int n, int K, Keep keep) {
   constexpr int J = SEL_CAP / SEL_THREADS;
   uint64_t k[J];
 #pragma unroll
@@ -273,7 +276,7 @@ __device__ __forceinline__ uint64_t shrink(Selection& sel, int n, int K, Keep ke
 // raised to the K-th of those at hand and the groups are gone through again; the
 // keys of earlier groups (elements before `first`) stay.
 template <class T, bool CLEAN>
-__device__ __forceinline__ void drain(Selection& sel, int n, int K, int first, uint64_t& bound) {
+__device__ __forceinline__ void drain(Selection<T>& sel, int n, int K, int first, uint64_t& bound) {
   constexpr int N = Words<T>::N;
   for (bool again = true; again;) {
     for (int i = threadIdx.x; i < n; i += SEL_THREADS) {
@@ -308,28 +311,28 @@ __device__ __forceinline__ void drain(Selection& sel, int n, int K, int first, u
 // sorted. m is the slice's largest logit, s the sum. All SEL_THREADS threads; sel
 // is set up and not in use.
 template <class T, bool CLEAN>
-__device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int begin, int end, int K,
+__device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int begin, int end, int K,
                                              float c, float& m, double& s, uint32_t& parity,
                                              unsigned* err) {
-  constexpr int N = Words<T>::N;
+  constexpr int N = Words<T>::N, R = Selection<T>::R, CHUNK = Selection<T>::CHUNK;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool even = even_start(z);
   const int total = begin < end ? (end - begin + N - 1) / N : 0;  // words
-  const int chunks = (total + SEL_CHUNK - 1) / SEL_CHUNK;
+  const int chunks = (total + CHUNK - 1) / CHUNK;
   const T* zb = z + begin;
   const uint32_t skew = (uint32_t)((uintptr_t)zb & 15);  // of every chunk's first byte
   // A chunk comes through shared memory if the 16-byte pieces that cover it lie
   // inside the slice; the first one of an unaligned row and the last do not.
   auto staged = [&](int i) {
-    return (i > 0 || skew == 0) && (i + 1) * SEL_CHUNK * N + (skew ? 16 / (int)sizeof(T) : 0) <=
+    return (i > 0 || skew == 0) && (i + 1) * CHUNK * N + (skew ? 16 / (int)sizeof(T) : 0) <=
                                        end - begin;
   };
   auto fetch = [&](int i) {  // one thread
-    const uint32_t bytes = SEL_CHUNK * 4 + (skew ? 16 : 0);
+    const uint32_t bytes = CHUNK * 4 + (skew ? 16 : 0);
     uint64_t* bar = &sel.bar[i % SEL_STAGES];
     rnet_dev::mbar_arrive_expect_tx(bar, bytes);
     bulk_load(sel.ring[i % SEL_STAGES],
-              reinterpret_cast<const char*>(zb + (size_t)i * SEL_CHUNK * N) - skew, bytes, bar);
+              reinterpret_cast<const char*>(zb + (size_t)i * CHUNK * N) - skew, bytes, bar);
   };
   if (tid == 0) {
     sel.keys = sel.groups = 0;
@@ -344,8 +347,8 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
   int epoch = begin;        // the queue's elements lie behind this one
   m = -FLT_MAX;
   for (int i = 0; i < chunks; ++i) {
-    const int w0 = begin / N + i * SEL_CHUNK;  // the row's first word of the chunk
-    uint32_t w[SEL_R];
+    const int w0 = begin / N + i * CHUNK;  // the row's first word of the chunk
+    uint32_t w[R];
     if (staged(i)) {
       const int b = i % SEL_STAGES;
       // a copy that does not come is reported and given the same time once more:
@@ -356,11 +359,11 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
       const char* p = reinterpret_cast<const char*>(sel.ring[b]) + skew + 4 * tid;
       if (even) {
 #pragma unroll
-        for (int j = 0; j < SEL_R; ++j)
+        for (int j = 0; j < R; ++j)
           w[j] = *reinterpret_cast<const uint32_t*>(p + 4 * SEL_THREADS * j);
       } else {
 #pragma unroll
-        for (int j = 0; j < SEL_R; ++j) {
+        for (int j = 0; j < R; ++j) {
           const unsigned short* q =
               reinterpret_cast<const unsigned short*>(p + 4 * SEL_THREADS * j);
           w[j] = q[0] | (uint32_t)q[1] << 16;
@@ -368,22 +371,22 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < SEL_R; ++j)
+      for (int j = 0; j < R; ++j)
         w[j] = load_word(z, w0 + j * SEL_THREADS + tid, end, even);
     }
-    float top[SEL_R / SEL_GROUP];
+    float top[R / SEL_GROUP];
     float mine = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < SEL_R / SEL_GROUP; ++g) {
+    for (int g = 0; g < R / SEL_GROUP; ++g) {
       top[g] = words_max<T, SEL_GROUP, CLEAN>(w + g * SEL_GROUP);
       mine = fmaxf(mine, top[g]);
     }
     const float mx = fmaxf(m, mine);
-    sum = sum * exp2_fast((m - mx) * c) + words_sum<T, SEL_R, CLEAN>(w, mx, c);
+    sum = sum * exp2_fast((m - mx) * c) + words_sum<T, R, CLEAN>(w, mx, c);
     m = mx;
     if (i < 4 || (i & 3) == 0) {
       // K logits reach the least of the warps' r-th largest thread maxima so far
-      const float v = warp_nth(m, (K + SEL_WARPS - 1) / SEL_WARPS);
+      const float v = K <= SEL_WARPS ? warp_max(m) : warp_nth(m, (K + SEL_WARPS - 1) / SEL_WARPS);
       if (lane == 0) sel.bound[i & 1][warp] = v;
       __syncthreads();
       float least = sel.bound[i & 1][0];
@@ -415,7 +418,7 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
     bool full;
     auto queue = [&](auto wanted) {
 #pragma unroll
-      for (int g = 0; g < SEL_R / SEL_GROUP; ++g)
+      for (int g = 0; g < R / SEL_GROUP; ++g)
         if (top[g] >= lowest && wanted(g)) {
           const int at = atomicAdd(&sel.groups, 1);
           full |= at >= SEL_QUEUE - SEL_QUEUE / 4;
@@ -445,7 +448,7 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
         lowest = key_value(bound);
         exact = true;
         if (tid == 0) sel.groups = 0;
-        epoch = again ? here : here + SEL_CHUNK * N;
+        epoch = again ? here : here + CHUNK * N;
         __syncthreads();
       }
     }
@@ -485,7 +488,7 @@ __device__ __forceinline__ int cta_select_as(Selection& sel, const T* z, int beg
   return min(n, K);
 }
 template <class T>
-__device__ __forceinline__ int cta_select(Selection& sel, const T* z, int begin, int end, int K,
+__device__ __forceinline__ int cta_select(Selection<T>& sel, const T* z, int begin, int end, int K,
                                           float c, float& m, double& s, uint32_t& parity,
                                           unsigned* err) {
   int n = cta_select_as<T, false>(sel, z, begin, end, K, c, m, s, parity, err);
