@@ -249,44 +249,119 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(
       *reinterpret_cast<Vec*>(dst + base + j * pitch) = v[j];
 }
 
-// One CTA per sequence; thread j walks the parents of last beam j backwards.
-__global__ void __launch_bounds__(32) beam_backtrack_kernel(
+// ---------------------------------------------------------------- sequences
+// The way back from the last step is a chain of dependent looks at the parents.
+// It is cut into segments of steps, a warp each: a warp's lanes hold a step's
+// parents, so that a look is a shuffle and the loads do not wait for it. Each
+// warp first finds where every beam at its segment's end comes from; these maps
+// are chained, and the segments are walked again from the right beams, first for
+// the first eos, then to write. What bounds it is the latency of the shuffles of
+// one segment, three times.
+constexpr int BACK_UNROLL = 8;
+
+// Walks steps [begin, end) from the last to the first, for beam `a` of lane j at
+// step end - 1. f(t, a) sees the beam at each step. Returns the beam before the
+// segment.
+template <class F>
+__device__ __forceinline__ int walk(const int* parents, size_t M, size_t m0, int W, int begin,
+                                    int end, int a, bool& bad, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int t1 = end; t1 > begin; t1 -= BACK_UNROLL) {
+    int p[BACK_UNROLL];
+#pragma unroll
+    for (int i = 0; i < BACK_UNROLL; ++i) {
+      const int t = t1 - 1 - i;
+      p[i] = t >= begin && lane < W ? parents[(size_t)t * M + m0 + lane] : lane;
+      if (p[i] < 0 || p[i] >= (lane < W ? W : 32)) p[i] = lane, bad = true;
+    }
+    f(t1, a, p);
+#pragma unroll
+    for (int i = 0; i < BACK_UNROLL; ++i) a = __shfl_sync(~0u, p[i], a);
+  }
+  return a;
+}
+
+__global__ void __launch_bounds__(1024) beam_backtrack_kernel(
     const int* __restrict__ tokens, const int* __restrict__ parents,
     const float* __restrict__ scores, int eos, float alpha, int* __restrict__ seq,
-    int* __restrict__ lengths, float* __restrict__ ranked, int T, int M, int W, unsigned* err) {
+    int* __restrict__ lengths, float* __restrict__ ranked, int T, size_t M, int W, int steps,
+    unsigned* err) {
   rnet_dev::pdl_trigger();
-  const int j = threadIdx.x;
+  __shared__ int from[32][33], ends[32][33];  // [segment][beam]
+  __shared__ int s_len[32], s_rank[32];
+  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5, segs = blockDim.x >> 5;
   const size_t m0 = (size_t)blockIdx.x * W;
-  int len = T;
+  const int begin = min(seg * steps, T), end = min(begin + steps, T);
   bool bad = false;
-  if (j < W) {
-    int a = j;
-    for (int t = T - 1; t >= 0; --t) {
-      const size_t at = (size_t)t * M + m0 + a;
-      if (eos >= 0 && tokens[at] == eos) len = t + 1;
-      const int p = parents[at];
-      bad |= p < 0 || p >= W;
-      a = p < 0 || p >= W ? a : p;
+  from[seg][lane] = walk(parents, M, m0, W, begin, end, lane, bad, [](int, int, const int*) {});
+  if (bad && err) atomicOr(err, rnet_dev::ERR_BAD_INDEX);
+  __syncthreads();
+  if (seg == 0) {
+    int a = lane;
+    for (int k = segs - 1; k >= 0; --k) {
+      const int next = from[k][a];
+      __syncwarp();
+      from[k][lane] = a;  // where the walk of this segment starts
+      a = next;
     }
   }
-  if (bad && err) atomicOr(err, rnet_dev::ERR_BAD_INDEX);
-  double r = -INFINITY;
-  if (j < W) r = (double)canon(scores[m0 + j]) / pow((double)(len > 0 ? len : 1), (double)alpha);
-  int rank = 0;
-  for (int i = 0; i < W; ++i) {
-    const double o = __shfl_sync(~0u, r, i);
-    rank += o > r || (o == r && i < j);
+  __syncthreads();
+  const int start = from[seg][lane];
+  // tokens of BACK_UNROLL steps below t1 along the way
+  auto take = [&](int t1, int a, const int* p, int* out) {
+    int v[BACK_UNROLL];
+#pragma unroll
+    for (int i = 0; i < BACK_UNROLL; ++i) {
+      const int t = t1 - 1 - i;
+      v[i] = t >= begin && lane < W ? tokens[(size_t)t * M + m0 + lane] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < BACK_UNROLL; ++i) {
+      out[i] = __shfl_sync(~0u, v[i], a);
+      a = __shfl_sync(~0u, p[i], a);
+    }
+  };
+  int len = T;
+  if (eos >= 0) {
+    walk(parents, M, m0, W, begin, end, start, bad, [&](int t1, int a, const int* p) {
+      int v[BACK_UNROLL];
+      take(t1, a, p, v);
+#pragma unroll
+      for (int i = 0; i < BACK_UNROLL; ++i)
+        if (t1 - 1 - i >= begin && v[i] == eos) len = t1 - i;
+    });
+    ends[seg][lane] = len;
+    __syncthreads();
   }
-  if (j >= W) return;
-  lengths[m0 + rank] = len;
-  ranked[m0 + rank] = (float)r;
-  int a = j;
-  for (int t = T - 1; t >= 0; --t) {
-    const size_t at = (size_t)t * M + m0 + a;
-    seq[(m0 + rank) * T + t] = t >= len ? eos : tokens[at];
-    const int p = parents[at];
-    a = p < 0 || p >= W ? a : p;
+  if (seg == 0) {
+    if (eos >= 0)
+      for (int k = 0; k < segs; ++k) len = min(len, ends[k][lane]);
+    const double r = lane < W ? (double)canon(scores[m0 + lane]) / pow((double)len, (double)alpha)
+                              : -(double)INFINITY;
+    int rank = 0;
+    for (int i = 0; i < W; ++i) {
+      const double o = __shfl_sync(~0u, r, i);
+      rank += o > r || (o == r && i < lane);
+    }
+    s_len[lane] = len;
+    s_rank[lane] = rank;
+    if (lane < W) {
+      lengths[m0 + rank] = len;
+      ranked[m0 + rank] = (float)r;
+    }
   }
+  __syncthreads();
+  len = s_len[lane];
+  int* out = seq + (m0 + (lane < W ? s_rank[lane] : 0)) * T;
+  walk(parents, M, m0, W, begin, end, start, bad, [&](int t1, int a, const int* p) {
+    int v[BACK_UNROLL];
+    take(t1, a, p, v);
+#pragma unroll
+    for (int i = 0; i < BACK_UNROLL; ++i) {
+      const int t = t1 - 1 - i;
+      if (lane < W && t >= begin) out[t] = t >= len ? eos : v[i];
+    }
+  });
 }
 
 template <class Vec>
@@ -335,8 +410,13 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
                            float alpha, int* sequences, int* lengths, float* ranked, int steps,
                            int batch, int beams, unsigned* err, cudaStream_t s) {
   if (batch <= 0) return cudaSuccess;
-  beam_backtrack_kernel<<<batch, 32, 0, s>>>(tokens, parents, scores, eos, alpha, sequences,
-                                             lengths, ranked, steps, batch * beams, beams, err);
+  // segments of at least 16 steps, 32 of them at most
+  int segs = (steps + 15) / 16;
+  if (segs > 32) segs = 32;
+  const int per = (steps + segs - 1) / segs;
+  beam_backtrack_kernel<<<batch, 32 * segs, 0, s>>>(tokens, parents, scores, eos, alpha, sequences,
+                                                    lengths, ranked, steps, (size_t)batch * beams,
+                                                    beams, per, err);
   return launched();
 }
 
