@@ -251,97 +251,110 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(
 
 // ---------------------------------------------------------------- sequences
 // The way back from the last step is a chain of dependent looks at the parents.
-// It is cut into segments of steps, a warp each: a warp's lanes hold a step's
-// parents, so that a look is a shuffle and the loads do not wait for it. Each
-// warp first finds where every beam at its segment's end comes from; these maps
-// are chained, and the segments are walked again from the right beams, first for
-// the first eos, then to write. What bounds it is the latency of the shuffles of
-// one segment, three times.
-constexpr int BACK_UNROLL = 8;
+// It is cut into segments of steps, and a lane walks a segment for a beam: 32 / P
+// segments in a warp (P = beams, rounded up to a power of two), so that a look is
+// a shuffle inside P lanes and the loads do not wait for it. Each segment first
+// finds where every beam at its end comes from; these maps are chained over the
+// segments of a warp, then over the warps, and the segments are walked again from
+// the right beams, first for the first eos, then to write. What bounds it is the
+// latency of one segment's loads and shuffles, three times.
+constexpr int BACK_WARPS = 32;
+constexpr int BACK = 8;  // steps whose loads are under way together
 
-// Walks steps [begin, end) from the last to the first, for beam `a` of lane j at
-// step end - 1. f(t, a) sees the beam at each step. Returns the beam before the
-// segment.
-template <class F>
-__device__ __forceinline__ int walk(const int* parents, size_t M, size_t m0, int W, int begin,
-                                    int end, int a, bool& bad, F f) {
-  const int lane = threadIdx.x & 31;
-  for (int t1 = end; t1 > begin; t1 -= BACK_UNROLL) {
-    int p[BACK_UNROLL];
+struct Segment {
+  const int *parents, *tokens;  // of this lane's beam
+  size_t M;
+  int begin, end;  // steps
+  int first;       // lane of the segment's beam 0
+  int W;
+  bool on;         // this lane has a beam
+
+  // From beam a at step end - 1 to the first step; f(t, token) sees the tokens on
+  // the way. Returns the beam before the segment. `steps` is the same in all lanes.
+  template <bool TOKENS, class F>
+  __device__ __forceinline__ int walk(int steps, int a, bool& bad, F f) const {
+    const int own = (threadIdx.x & 31) - first;
+    for (int k = 0; k < steps; k += BACK) {
+      int p[BACK], v[BACK];
 #pragma unroll
-    for (int i = 0; i < BACK_UNROLL; ++i) {
-      const int t = t1 - 1 - i;
-      p[i] = t >= begin && lane < W ? parents[(size_t)t * M + m0 + lane] : lane;
-      if (p[i] < 0 || p[i] >= (lane < W ? W : 32)) p[i] = lane, bad = true;
+      for (int i = 0; i < BACK; ++i) {
+        const int t = end - 1 - k - i;
+        const bool in = on && t >= begin;
+        p[i] = in ? parents[(size_t)t * M] : own;
+        if (TOKENS) v[i] = in ? tokens[(size_t)t * M] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < BACK; ++i) {
+        if (on && (p[i] < 0 || p[i] >= W)) p[i] = own, bad = true;
+        if (TOKENS) {
+          const int t = end - 1 - k - i, token = __shfl_sync(~0u, v[i], first + a);
+          if (t >= begin) f(t, token);
+        }
+        a = __shfl_sync(~0u, p[i], first + a);
+      }
     }
-    f(t1, a, p);
-#pragma unroll
-    for (int i = 0; i < BACK_UNROLL; ++i) a = __shfl_sync(~0u, p[i], a);
+    return a;
   }
-  return a;
-}
+};
 
-__global__ void __launch_bounds__(1024) beam_backtrack_kernel(
+__global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
     const int* __restrict__ tokens, const int* __restrict__ parents,
     const float* __restrict__ scores, int eos, float alpha, int* __restrict__ seq,
-    int* __restrict__ lengths, float* __restrict__ ranked, int T, size_t M, int W, int steps,
-    unsigned* err) {
+    int* __restrict__ lengths, float* __restrict__ ranked, int T, size_t M, int W, int P,
+    int steps, unsigned* err) {
   rnet_dev::pdl_trigger();
-  __shared__ int from[32][33], ends[32][33];  // [segment][beam]
+  __shared__ int map[BACK_WARPS][32], from[BACK_WARPS][32], ends[BACK_WARPS][32];
   __shared__ int s_len[32], s_rank[32];
-  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5, segs = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int G = 32 / P, beam = lane & (P - 1), part = lane / P;
   const size_t m0 = (size_t)blockIdx.x * W;
-  const int begin = min(seg * steps, T), end = min(begin + steps, T);
+  Segment sg;
+  sg.M = M;
+  sg.W = W;
+  sg.first = lane - beam;
+  sg.on = beam < W;
+  sg.begin = min((warp * G + part) * steps, T);
+  sg.end = min(sg.begin + steps, T);
+  sg.parents = parents + m0 + beam;
+  sg.tokens = tokens + m0 + beam;
   bool bad = false;
-  from[seg][lane] = walk(parents, M, m0, W, begin, end, lane, bad, [](int, int, const int*) {});
+  const int before = sg.walk<false>(steps, beam, bad, [](int, int) {});
   if (bad && err) atomicOr(err, rnet_dev::ERR_BAD_INDEX);
+  // this segment's start for every beam at the end of the warp's last segment
+  int a = beam, start = beam;
+  for (int g = G - 1; g >= 0; --g) {
+    if (part == g) start = a;
+    a = __shfl_sync(~0u, before, g * P + a);
+  }
+  map[warp][lane] = a;  // the same in all parts
   __syncthreads();
-  if (seg == 0) {
-    int a = lane;
-    for (int k = segs - 1; k >= 0; --k) {
-      const int next = from[k][a];
-      __syncwarp();
-      from[k][lane] = a;  // where the walk of this segment starts
-      a = next;
+  if (warp == 0) {
+    int b = beam;
+    for (int k = warps - 1; k >= 0; --k) {
+      from[k][lane] = b;
+      b = map[k][b];
     }
   }
   __syncthreads();
-  const int start = from[seg][lane];
-  // tokens of BACK_UNROLL steps below t1 along the way
-  auto take = [&](int t1, int a, const int* p, int* out) {
-    int v[BACK_UNROLL];
-#pragma unroll
-    for (int i = 0; i < BACK_UNROLL; ++i) {
-      const int t = t1 - 1 - i;
-      v[i] = t >= begin && lane < W ? tokens[(size_t)t * M + m0 + lane] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < BACK_UNROLL; ++i) {
-      out[i] = __shfl_sync(~0u, v[i], a);
-      a = __shfl_sync(~0u, p[i], a);
-    }
-  };
+  start = __shfl_sync(~0u, start, sg.first + from[warp][beam]);
   int len = T;
   if (eos >= 0) {
-    walk(parents, M, m0, W, begin, end, start, bad, [&](int t1, int a, const int* p) {
-      int v[BACK_UNROLL];
-      take(t1, a, p, v);
-#pragma unroll
-      for (int i = 0; i < BACK_UNROLL; ++i)
-        if (t1 - 1 - i >= begin && v[i] == eos) len = t1 - i;
+    sg.walk<true>(steps, start, bad, [&](int t, int token) {
+      if (token == eos) len = t + 1;
     });
-    ends[seg][lane] = len;
+    for (int o = P; o < 32; o <<= 1) len = min(len, __shfl_xor_sync(~0u, len, o));
+    ends[warp][lane] = len;
     __syncthreads();
   }
-  if (seg == 0) {
+  if (warp == 0) {
     if (eos >= 0)
-      for (int k = 0; k < segs; ++k) len = min(len, ends[k][lane]);
-    const double r = lane < W ? (double)canon(scores[m0 + lane]) / pow((double)len, (double)alpha)
-                              : -(double)INFINITY;
+      for (int k = 0; k < warps; ++k) len = min(len, ends[k][lane]);
+    const double r = sg.on ? (double)canon(scores[m0 + beam]) / pow((double)len, (double)alpha)
+                           : -(double)INFINITY;
     int rank = 0;
     for (int i = 0; i < W; ++i) {
       const double o = __shfl_sync(~0u, r, i);
-      rank += o > r || (o == r && i < lane);
+      rank += o > r || (o == r && i < beam);
     }
     s_len[lane] = len;
     s_rank[lane] = rank;
@@ -351,16 +364,10 @@ __global__ void __launch_bounds__(1024) beam_backtrack_kernel(
     }
   }
   __syncthreads();
-  len = s_len[lane];
-  int* out = seq + (m0 + (lane < W ? s_rank[lane] : 0)) * T;
-  walk(parents, M, m0, W, begin, end, start, bad, [&](int t1, int a, const int* p) {
-    int v[BACK_UNROLL];
-    take(t1, a, p, v);
-#pragma unroll
-    for (int i = 0; i < BACK_UNROLL; ++i) {
-      const int t = t1 - 1 - i;
-      if (lane < W && t >= begin) out[t] = t >= len ? eos : v[i];
-    }
+  len = s_len[beam];
+  int* out = seq + (m0 + (sg.on ? s_rank[beam] : 0)) * T;
+  sg.walk<true>(steps, start, bad, [&](int t, int token) {
+    if (sg.on) out[t] = t >= len ? eos : token;
   });
 }
 
@@ -410,13 +417,16 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
                            float alpha, int* sequences, int* lengths, float* ranked, int steps,
                            int batch, int beams, unsigned* err, cudaStream_t s) {
   if (batch <= 0) return cudaSuccess;
-  // segments of at least 16 steps, 32 of them at most
-  int segs = (steps + 15) / 16;
-  if (segs > 32) segs = 32;
-  const int per = (steps + segs - 1) / segs;
-  beam_backtrack_kernel<<<batch, 32 * segs, 0, s>>>(tokens, parents, scores, eos, alpha, sequences,
-                                                    lengths, ranked, steps, (size_t)batch * beams,
-                                                    beams, per, err);
+  int P = 1;
+  while (P < beams) P *= 2;
+  // segments of at least BACK steps
+  const int per_warp = 32 / P;
+  int warps = (steps + BACK * per_warp - 1) / (BACK * per_warp);
+  if (warps > BACK_WARPS) warps = BACK_WARPS;
+  const int per = (steps + warps * per_warp - 1) / (warps * per_warp);
+  beam_backtrack_kernel<<<batch, 32 * warps, 0, s>>>(tokens, parents, scores, eos, alpha,
+                                                     sequences, lengths, ranked, steps,
+                                                     (size_t)batch * beams, beams, P, per, err);
   return launched();
 }
 
