@@ -341,8 +341,21 @@ int rnet_model_step(rnet_model* m, float lr, float grad_clip);
  * buffers may differ from call to call. */
 int rnet_model_train_step(rnet_model* m, const int* d_inputs, const int* d_targets, int batch,
                           int seq_len, float lr, float grad_clip, float* d_loss_sum);
-/* Same with host token buffers; copies in, steps, copies the loss sum out and
- * waits for it. */
+/* The same step with rnet_distill_topk_forward's loss in the place of the
+ * cross-entropy: the teacher's records d_teacher_idx / d_teacher_logits
+ * [batch * seq_len, top_k], d_teacher_lse (may be NULL), d_targets (may be NULL
+ * without hard_weight) and d_row_weight (may be NULL) as there, all device
+ * pointers; dlogits scaled by 1/(batch*seq_len), d_loss_sum (may be NULL) the
+ * sum of the rows' losses. Runs on the model stream, always eager (no graph).
+ * No counterpart in the reference. */
+int rnet_model_train_step_distill(rnet_model* m, const int* d_inputs, const int* d_teacher_idx,
+                                  const float* d_teacher_logits, const float* d_teacher_lse,
+                                  const int* d_targets, const float* d_row_weight, int batch,
+                                  int seq_len, int top_k, float temperature, float soft_weight,
+                                  float hard_weight, float lr, float grad_clip,
+                                  float* d_loss_sum);
+/* Same as rnet_model_train_step with host token buffers; copies in, steps,
+ * copies the loss sum out and waits for it. */
 int rnet_model_train_step_host(rnet_model* m, const int* h_inputs, const int* h_targets,
                                int batch, int seq_len, float lr, float grad_clip,
                                float* h_loss_sum);
@@ -390,6 +403,22 @@ int rnet_decoder_destroy(rnet_decoder* d);
  * folds the slot keys / values with proj_q / proj_out for the decode steps,
  * from the weights of this moment: prefill again after changing weights. */
 int rnet_decoder_prefill(rnet_decoder* d, const int* d_tokens, int seq_len);
+/* Prefill for a beam search: d_tokens [n_streams / beams, seq_len], one prompt
+ * per sequence; its `beams` streams (in a row) all start from its state. */
+int rnet_decoder_prefill_beams(rnet_decoder* d, const int* d_tokens, int seq_len, int beams);
+/* Beam search of n_steps tokens from the current logits and states (after a
+ * prefill): n_streams / beams sequences of `beams` streams each, beams 1..32
+ * dividing n_streams; a sequence starts from its first stream. Per step:
+ * rnet_beam_select on the logits, rnet_beam_reorder of the recurrent states by
+ * the parents, one decode step. eos = -1: no token ends a beam. Outputs (device)
+ * as rnet_beam_backtrack with n_steps: d_sequences [n_streams, n_steps],
+ * d_lengths and d_scores [n_streams], ranked per sequence by
+ * score / length^length_alpha. use_graph = 1 replays one captured CUDA graph per
+ * step. Asynchronous on the model stream, except that it waits when the record
+ * of steps has to grow. Afterwards the streams hold the beams of the last
+ * selection, unranked, and rnet_decoder_step(d, NULL) feeds their last tokens. */
+int rnet_decoder_beam_search(rnet_decoder* d, int beams, int n_steps, int eos, float length_alpha,
+                             int* d_sequences, int* d_lengths, float* d_scores, int use_graph);
 /* One token per stream: d_tokens [n_streams] (device) or NULL to feed back
  * the previous argmax. */
 int rnet_decoder_step(rnet_decoder* d, const int* d_tokens);

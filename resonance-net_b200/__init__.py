@@ -98,6 +98,7 @@ _SIGS = {
     "rnet_model_zero_grad": [_P],
     "rnet_model_step": [_P, _F, _F],
     "rnet_model_train_step": [_P, _P, _P, _I, _I, _F, _F, _P],
+    "rnet_model_train_step_distill": [_P] * 7 + [_I, _I, _I] + [_F] * 5 + [_P],
     "rnet_model_train_step_host": [_P, _P, _P, _I, _I, _F, _F, ctypes.POINTER(_F)],
     "rnet_model_topk": [_P, _I, ctypes.POINTER(_P), ctypes.POINTER(_P)],
     "rnet_model_topk_host": [_P, _I, _P, _P, _SZ],
@@ -112,6 +113,8 @@ _SIGS = {
     "rnet_decoder_create": [_P, _I, ctypes.POINTER(_P)],
     "rnet_decoder_destroy": [_P],
     "rnet_decoder_prefill": [_P, _P, _I],
+    "rnet_decoder_prefill_beams": [_P, _P, _I, _I],
+    "rnet_decoder_beam_search": [_P, _I, _I, _I, _F, _P, _P, _P, _I],
     "rnet_decoder_step": [_P, _P],
     "rnet_decoder_generate": [_P, _I, _P, _I],
     "rnet_decoder_set_sampling": [_P, _F, _F, ctypes.c_ulonglong],
@@ -282,6 +285,17 @@ class Model:
         check(lib().rnet_model_train_step(self._h, _ptr(d_in), _ptr(d_tgt), batch, seq_len, lr,
                                           clip, _ptr(d_loss_sum)))
 
+    def train_step_distill(self, d_in, d_teacher_idx, d_teacher_logits, batch: int, seq_len: int,
+                           top_k: int, temperature: float = 1.0, soft_weight: float = 1.0,
+                           hard_weight: float = 0.0, d_tgt=None, d_teacher_lse=None,
+                           d_row_weight=None, lr: float = 3e-4, clip: float = 1.0,
+                           d_loss_sum=None) -> None:
+        """A step on a teacher's top-logit records (rnet_topk_logits_forward)."""
+        check(lib().rnet_model_train_step_distill(
+            self._h, _ptr(d_in), _ptr(d_teacher_idx), _ptr(d_teacher_logits), _ptr(d_teacher_lse),
+            _ptr(d_tgt), _ptr(d_row_weight), batch, seq_len, top_k, temperature, soft_weight,
+            hard_weight, lr, clip, _ptr(d_loss_sum)))
+
     def train_step_host(self, h_in, h_tgt, batch: int, seq_len: int, lr: float = 3e-4,
                         clip: float = 1.0) -> float:
         loss = _F()
@@ -346,6 +360,18 @@ class Decoder:
 
     def prefill(self, d_tokens, seq_len: int) -> None:
         check(lib().rnet_decoder_prefill(self.handle, _ptr(d_tokens), seq_len))
+
+    def prefill_beams(self, d_tokens, seq_len: int, beams: int) -> None:
+        """One prompt per `beams` streams: d_tokens [n_streams / beams, seq_len]."""
+        check(lib().rnet_decoder_prefill_beams(self.handle, _ptr(d_tokens), seq_len, beams))
+
+    def beam_search(self, beams: int, n_steps: int, d_sequences, d_lengths, d_scores,
+                    eos: int = -1, length_alpha: float = 0.0, use_graph: bool = True) -> None:
+        """Beam search after a prefill: d_sequences [n_streams, n_steps] int32, d_lengths
+        [n_streams] int32 and d_scores [n_streams] float32, best first per sequence."""
+        check(lib().rnet_decoder_beam_search(self.handle, beams, n_steps, eos, length_alpha,
+                                             _ptr(d_sequences), _ptr(d_lengths), _ptr(d_scores),
+                                             int(use_graph)))
 
     def step(self, d_tokens=None) -> None:
         check(lib().rnet_decoder_step(self.handle, _ptr(d_tokens)))

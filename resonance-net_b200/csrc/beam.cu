@@ -371,6 +371,33 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
   });
 }
 
+// ---------------------------------------------------------------- a search's records
+__global__ void beam_begin_kernel(float* scores, int* finished, int* step, int M, int W) {
+  rnet_dev::pdl_trigger();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i == 0) *step = 0;
+  if (i >= M) return;
+  scores[i] = i % W ? -INFINITY : 0.f;
+  finished[i] = 0;
+}
+
+// One CTA: the row is known to all threads before the first one moves it on.
+__global__ void __launch_bounds__(1024) beam_record_kernel(const int* tokens, const int* parents,
+                                                           int* hist_tokens, int* hist_parents,
+                                                           int M, int* step, int* pos) {
+  rnet_dev::pdl_trigger();
+  const int row = *step;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *step = row + 1;
+    if (row) *pos += 1;
+  }
+  for (int i = threadIdx.x; i < M; i += 1024) {
+    hist_tokens[(size_t)row * M + i] = tokens[i];
+    hist_parents[(size_t)row * M + i] = parents[i];
+  }
+}
+
 template <class Vec>
 cudaError_t reorder_as(const char* src, char* dst, size_t row_bytes, size_t pitch, size_t outer,
                        size_t outer_pitch, const int* parents, int batch, int beams, unsigned* err,
@@ -411,6 +438,19 @@ cudaError_t beam_reorder(const void* src, void* dst, size_t row_bytes, size_t pi
                              err, s);
   return reorder_as<uint32_t>(a, b, row_bytes, pitch, outer, outer_pitch, parents, batch, beams,
                               err, s);
+}
+
+cudaError_t beam_begin(float* scores, int* finished, int* step, int batch, int beams,
+                       cudaStream_t s) {
+  const int M = batch * beams;
+  beam_begin_kernel<<<(M + 255) / 256, 256, 0, s>>>(scores, finished, step, M, beams);
+  return launched();
+}
+
+cudaError_t beam_record(const int* tokens, const int* parents, int* hist_tokens,
+                        int* hist_parents, int M, int* step, int* pos, cudaStream_t s) {
+  beam_record_kernel<<<1, 1024, 0, s>>>(tokens, parents, hist_tokens, hist_parents, M, step, pos);
+  return launched();
 }
 
 cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,

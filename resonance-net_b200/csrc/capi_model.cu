@@ -2,6 +2,7 @@
 #include <sys/stat.h>
 
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <new>
 #include <string>
@@ -9,6 +10,7 @@
 
 #include "dist.h"
 #include "engine.h"
+#include "kernels.cuh"
 #include "status.h"
 
 using rnet_engine::Engine;
@@ -187,6 +189,30 @@ int rnet_model_train_step(rnet_model* m, const int* d_inputs, const int* d_targe
   return m->e->train_step(d_inputs, d_targets, batch, seq_len, lr, grad_clip, d_loss_sum);
 }
 
+int rnet_model_train_step_distill(rnet_model* m, const int* d_inputs, const int* d_teacher_idx,
+                                  const float* d_teacher_logits, const float* d_teacher_lse,
+                                  const int* d_targets, const float* d_row_weight, int batch,
+                                  int seq_len, int top_k, float temperature, float soft_weight,
+                                  float hard_weight, float lr, float grad_clip,
+                                  float* d_loss_sum) {
+  CHECK_M(m);
+  if (!d_inputs || !d_teacher_idx || !d_teacher_logits)
+    return rnet_status::fail(RNET_ERR_ARG, "train_step_distill: null pointer");
+  if (top_k < 1 || top_k > RNET_TOPK_MAX)
+    return rnet_status::fail(RNET_ERR_ARG, "train_step_distill: top_k must be 1.." +
+                                               std::to_string(RNET_TOPK_MAX));
+  if (!(temperature >= 1e-4f && temperature <= 1e4f))
+    return rnet_status::fail(RNET_ERR_ARG,
+                             "train_step_distill: temperature must be within 1e-4 and 1e4");
+  if (!std::isfinite(soft_weight) || !std::isfinite(hard_weight))
+    return rnet_status::fail(RNET_ERR_ARG, "train_step_distill: weights must be finite");
+  if (hard_weight != 0.0f && !d_targets)
+    return rnet_status::fail(RNET_ERR_ARG, "train_step_distill: hard_weight needs targets");
+  return m->e->train_step_distill(d_inputs, d_teacher_idx, d_teacher_logits, d_teacher_lse,
+                                  d_targets, d_row_weight, batch, seq_len, top_k, temperature,
+                                  soft_weight, hard_weight, lr, grad_clip, d_loss_sum);
+}
+
 int rnet_model_train_step_host(rnet_model* m, const int* h_inputs, const int* h_targets,
                                int batch, int seq_len, float lr, float grad_clip,
                                float* h_loss_sum) {
@@ -300,6 +326,27 @@ int rnet_decoder_destroy(rnet_decoder* d) {
 int rnet_decoder_prefill(rnet_decoder* d, const int* d_tokens, int seq_len) {
   if (!d || !d_tokens) return rnet_status::fail(RNET_ERR_ARG, "null argument");
   return d->m->e->prefill(&d->d, d_tokens, seq_len);
+}
+
+int rnet_decoder_prefill_beams(rnet_decoder* d, const int* d_tokens, int seq_len, int beams) {
+  if (!d || !d_tokens) return rnet_status::fail(RNET_ERR_ARG, "null argument");
+  return d->m->e->prefill(&d->d, d_tokens, seq_len, beams);
+}
+
+int rnet_decoder_beam_search(rnet_decoder* d, int beams, int n_steps, int eos, float length_alpha,
+                             int* d_sequences, int* d_lengths, float* d_scores, int use_graph) {
+  if (!d || !d_sequences || !d_lengths || !d_scores)
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: null argument");
+  if (beams < 1 || beams > RNET_BEAMS_MAX)
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: beams must be 1.." +
+                                               std::to_string(RNET_BEAMS_MAX));
+  if (n_steps < 1) return rnet_status::fail(RNET_ERR_ARG, "beam_search: n_steps must be >= 1");
+  if (eos < -1 || eos >= d->m->e->config().vocab_size)
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: eos must be -1 (none) or a token");
+  if (!std::isfinite(length_alpha))
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: length_alpha must be finite");
+  return d->m->e->beam_search(&d->d, beams, n_steps, eos, length_alpha, d_sequences, d_lengths,
+                              d_scores, use_graph != 0);
 }
 
 int rnet_decoder_step(rnet_decoder* d, const int* d_tokens) {

@@ -34,32 +34,33 @@ __global__ void decode_conv_kernel(const float* __restrict__ n, float* __restric
       rnet_dev::conv_step4(x, ring + (size_t)m * RING * D, *pos_ptr, w3, w7, w15, d, D);
 }
 
-// After a prefill of T steps: h_state[m] = h[m, T-1]; ring[t % 14] = n1[m, t]
-// for t in [T-14, T-1] (zero for t < 0).
+// After a prefill of T steps: h_state[m] = h[r, T-1]; ring[t % 14] = n1[r, t]
+// for t in [T-14, T-1] (zero for t < 0), with r = m / copies (copies streams
+// start from each prompt).
 __global__ void extract_state_kernel(const float* __restrict__ n1, const float* __restrict__ h,
                                      float* __restrict__ ring, float* __restrict__ hs, int M,
-                                     int T, int D) {
+                                     int T, int D, int copies) {
   rnet_dev::pdl_trigger();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= M * D) return;
-  const int m = i / D, d = i % D;
-  hs[i] = h[((size_t)m * T + T - 1) * D + d];
+  const int m = i / D, d = i % D, r = m / copies;
+  hs[i] = h[((size_t)r * T + T - 1) * D + d];
   float* rg = ring + (size_t)m * RING * D + d;
   for (int j = 0; j < RING; ++j) {
     const int t = T - RING + j;
-    if (t >= 0) rg[(size_t)(t % RING) * D] = n1[((size_t)m * T + t) * D + d];
+    if (t >= 0) rg[(size_t)(t % RING) * D] = n1[((size_t)r * T + t) * D + d];
     else rg[(size_t)(((t % RING) + RING) % RING) * D] = 0.f;
   }
 }
 
-// Row gather: out[m] = x[m*T + T-1]
+// Row gather: out[m] = x[r*T + T-1], r = m / copies
 __global__ void last_rows_kernel(const float* __restrict__ x, float* __restrict__ out, int M,
-                                 int T, int D) {
+                                 int T, int D, int copies) {
   rnet_dev::pdl_trigger();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= M * D) return;
-  const int m = i / D, d = i % D;
-  out[i] = x[((size_t)m * T + T - 1) * D + d];
+  const int m = i / D, d = i % D, r = m / copies;
+  out[i] = x[((size_t)r * T + T - 1) * D + d];
 }
 
 // Greedy argmax per row (first maximum wins), one warp per row; writes the
@@ -440,13 +441,14 @@ cudaError_t decode_conv(const float* n, float* ring, const int* pos, const float
 }
 
 cudaError_t decode_extract_state(const float* n1, const float* h, float* ring, float* hs, int M,
-                                 int T, int D, cudaStream_t s) {
-  extract_state_kernel<<<(M * D + 255) / 256, 256, 0, s>>>(n1, h, ring, hs, M, T, D);
+                                 int T, int D, cudaStream_t s, int copies) {
+  extract_state_kernel<<<(M * D + 255) / 256, 256, 0, s>>>(n1, h, ring, hs, M, T, D, copies);
   return launched();
 }
 
-cudaError_t last_rows(const float* x, float* out, int M, int T, int D, cudaStream_t s) {
-  last_rows_kernel<<<(M * D + 255) / 256, 256, 0, s>>>(x, out, M, T, D);
+cudaError_t last_rows(const float* x, float* out, int M, int T, int D, cudaStream_t s,
+                      int copies) {
+  last_rows_kernel<<<(M * D + 255) / 256, 256, 0, s>>>(x, out, M, T, D, copies);
   return launched();
 }
 

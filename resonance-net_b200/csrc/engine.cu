@@ -72,6 +72,7 @@ Engine::~Engine() {
   if (train_exec_) cudaGraphExecDestroy(train_exec_);
   cudaFree(g_in_);
   cudaFree(g_tgt_);
+  cudaFree(row_loss_);
   cudaFree(snap_);
   if (snap_host_) cudaFreeHost(snap_host_);
   if (snap_ready_) cudaEventDestroy(snap_ready_);
@@ -832,6 +833,38 @@ int Engine::train_step_eager(const int* d_in, const int* d_tgt, int B, int T, fl
   return step(lr, clip);
 }
 
+int Engine::train_step_distill(const int* d_in, const int* t_idx, const float* t_val,
+                               const float* t_lse, const int* d_tgt, const float* row_weight,
+                               int B, int T, int top_k, float tau, float soft, float hard,
+                               float lr, float clip, float* d_loss_sum) {
+  const long long tokens = (long long)B * T;
+  if (B <= 0 || T <= 0 || tokens > 64LL * (cfg_.seq_len > 0 ? cfg_.seq_len : 256))
+    return rnet_status::fail(RNET_ERR_ARG,
+                             "train_step_distill: batch*seq_len must be 1..64*seq_len");
+  const int N = (int)tokens, V = cfg_.vocab_size;
+  if (N > row_loss_cap_) {
+    CK(cudaStreamSynchronize(stream_));
+    cudaFree(row_loss_);
+    row_loss_ = nullptr;
+    row_loss_cap_ = 0;
+    CK(cudaMalloc(&row_loss_, N * sizeof(float)));
+    row_loss_cap_ = N;
+  }
+  int rc = zero_grad();
+  if (rc) return rc;
+  rc = ensure_capacity(N, true);
+  if (rc) return rc;
+  rc = forward(d_in, logits_, B, T);
+  if (rc) return rc;
+  PROF(PK_CE, 0, 8.0 * N * V + 8.0 * N * top_k,
+       rnet_k::distill_topk(logits_, false, V, t_idx, t_val, t_lse, d_tgt, row_weight, tau, soft,
+                            hard, 1.0f / (float)N, row_loss_, d_loss_sum ? d_loss_sum : loss_dev_,
+                            dlogits_, V, N, V, top_k, rnet_status::device_error_word(), stream_));
+  rc = backward(dlogits_, d_in, B, T);
+  if (rc) return rc;
+  return step(lr, clip);
+}
+
 // ------------------------------------------------------------------ decode
 int Engine::decoder_init(Decoder* d, int M) {
   if (M <= 0) return rnet_status::fail(RNET_ERR_ARG, "decoder: n_streams must be > 0");
@@ -873,16 +906,22 @@ int Engine::decoder_init(Decoder* d, int M) {
 void Engine::decoder_free(Decoder* d) {
   if (d->exec) cudaGraphExecDestroy(d->exec);
   if (d->graph) cudaGraphDestroy(d->graph);
+  if (d->beam.exec) cudaGraphExecDestroy(d->beam.exec);
   cudaStreamSynchronize(stream_);
+  cudaFree(d->beam.arena);
+  cudaFree(d->beam.hist_tokens);
+  d->beam = Decoder::Beam();
   cudaFree(d->arena);
   d->arena = nullptr;
   d->exec = nullptr;
   d->graph = nullptr;
 }
 
-int Engine::prefill(Decoder* d, const int* d_tokens, int T) {
+int Engine::prefill(Decoder* d, const int* d_tokens, int T, int copies) {
   if (T <= 0) return rnet_status::fail(RNET_ERR_ARG, "prefill: empty prompt");
-  const int M = d->M, N = M * T, D = cfg_.d_model, V = cfg_.vocab_size;
+  if (copies <= 0 || d->M % copies)
+    return rnet_status::fail(RNET_ERR_ARG, "prefill: n_streams must be a multiple of beams");
+  const int M = d->M, rows = M / copies, N = rows * T, D = cfg_.d_model, V = cfg_.vocab_size;
   int rc = ensure_capacity(N, false);
   if (rc) return rc;
   cudaStream_t s = stream_;
@@ -892,11 +931,11 @@ int Engine::prefill(Decoder* d, const int* d_tokens, int T) {
   for (int l = 0; l < cfg_.n_layers; ++l) {
     const float* Xl = X_ + (size_t)(l & 1) * ND;
     float* Xn = X_ + (size_t)((l + 1) & 1) * ND;
-    rc = layer_forward(l, Xl, Xn, act_[0], M, T, false);
+    rc = layer_forward(l, Xl, Xn, act_[0], rows, T, false);
     if (rc) return rc;
     float* st = d->state + (size_t)l * d->floats_per_layer;
     CK(rnet_k::decode_extract_state(act_[0].n1, act_[0].h, st, st + (size_t)M * 14 * D, M, T, D,
-                                    s));
+                                    s, copies));
   }
   have_cache_ = false;
   // fold the slot path's fixed projections for the decode steps:
@@ -908,7 +947,7 @@ int Engine::prefill(Decoder* d, const int* d_tokens, int T) {
     CK(rnet_k::fold_rows(VT_ + o, W_[l].pout, 1, (size_t)D, d->VP + o, S, D, D, s));
   }
   const float* XL = X_ + (size_t)(cfg_.n_layers & 1) * ND;
-  CK(rnet_k::last_rows(XL, d->x, M, T, D, s));
+  CK(rnet_k::last_rows(XL, d->x, M, T, D, s, copies));
   CK(rnet_k::rms_norm_fwd(d->x, fnorm_, d->n, nullptr, M, D, cfg_.rms_eps, s));
   MM(M, V, D, kmaj(d->n, D), kmaj(outw_, D), epi_store(d->logits, V), 0);
   CK(cudaMemcpyAsync(d->pos, &T, sizeof(int), cudaMemcpyHostToDevice, s));
@@ -919,12 +958,22 @@ int Engine::prefill(Decoder* d, const int* d_tokens, int T) {
 }
 
 int Engine::decode_step(Decoder* d, const int* d_tokens) {
+  cudaStream_t s = stream_;
+  if (d_tokens)
+    CK(cudaMemcpyAsync(d->tok, d_tokens, d->M * sizeof(int), cudaMemcpyDeviceToDevice, s));
+  const int rc = decode_logits(d);
+  if (rc) return rc;
+  CK(rnet_k::sample_rows(d->logits, d->M, cfg_.vocab_size, d->temperature, d->top_p, d->seed,
+                         d->tok, d->pos, 1, s));
+  return RNET_OK;
+}
+
+int Engine::decode_logits(Decoder* d) {
   const int M = d->M, D = cfg_.d_model, F = cfg_.d_ff, S = cfg_.n_slots, V = cfg_.vocab_size;
   const int L = cfg_.n_layers;
   const float eps = cfg_.rms_eps;
   cudaStream_t s = stream_;
   unsigned* err = rnet_status::device_error_word();
-  if (d_tokens) CK(cudaMemcpyAsync(d->tok, d_tokens, M * sizeof(int), cudaMemcpyDeviceToDevice, s));
   CK(rnet_k::embed_fwd(d->tok, embed_, d->x, M, V, D, err, s));
   CK(rnet_k::rms_norm_fwd(d->x, W_[0].n1, d->n, nullptr, M, D, eps, s));
   // Every residual update also writes the next sublayer's RMSNorm of x into
@@ -996,8 +1045,6 @@ int Engine::decode_step(Decoder* d, const int* d_tokens) {
     }
   }
   MM(M, V, D, kmaj(d->n, D), kmaj(outw_, D), epi_store(d->logits, V), 0);
-  CK(rnet_k::sample_rows(d->logits, M, V, d->temperature, d->top_p, d->seed, d->tok, d->pos, 1,
-                         s));
   return RNET_OK;
 }
 
@@ -1036,6 +1083,105 @@ int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
       CK(cudaMemcpyAsync(d_out + (size_t)i * d->M, d->tok, d->M * sizeof(int),
                          cudaMemcpyDeviceToDevice, s));
   }
+  return RNET_OK;
+}
+
+int Engine::beam_reserve(Decoder* d, int n_steps) {
+  Decoder::Beam& b = d->beam;
+  const size_t m = d->M;
+  if (!b.arena) {
+    CK(cudaMalloc(&b.arena, (3 * m + 1) * sizeof(int)));
+    b.scores = (float*)b.arena;
+    b.finished = (int*)b.arena + m;
+    b.parents = (int*)b.arena + 2 * m;
+    b.step = (int*)b.arena + 3 * m;
+  }
+  if (n_steps > b.cap) {
+    // the captured step writes into the old history
+    if (b.exec) cudaGraphExecDestroy(b.exec);
+    b.exec = nullptr;
+    CK(cudaStreamSynchronize(stream_));
+    cudaFree(b.hist_tokens);
+    b.hist_tokens = b.hist_parents = nullptr;
+    b.cap = 0;
+    CK(cudaMalloc(&b.hist_tokens, 2 * (size_t)n_steps * m * sizeof(int)));
+    b.hist_parents = b.hist_tokens + (size_t)n_steps * m;
+    b.cap = n_steps;
+  }
+  return RNET_OK;
+}
+
+int Engine::beam_choose(Decoder* d, int beams, int eos) {
+  Decoder::Beam& b = d->beam;
+  const int M = d->M, D = cfg_.d_model, V = cfg_.vocab_size, L = cfg_.n_layers, groups = M / beams;
+  cudaStream_t s = stream_;
+  unsigned* err = rnet_status::device_error_word();
+  int* finished = eos >= 0 ? b.finished : nullptr;
+  CK(rnet_k::beam_select(d->logits, false, V, b.scores, finished, eos, b.scores, d->tok, b.parents,
+                         finished, groups, beams, V, err, s));
+  CK(rnet_k::beam_record(d->tok, b.parents, b.hist_tokens, b.hist_parents, M, b.step, d->pos, s));
+  // per layer: the ring [M][14][D], then h [M][D]
+  const size_t row = D * sizeof(float), layer = d->floats_per_layer * sizeof(float);
+  float* h = d->state + (size_t)M * 14 * D;
+  CK(rnet_k::beam_reorder(d->state, d->state, 14 * row, 14 * row, L, layer, b.parents, groups,
+                          beams, err, s));
+  CK(rnet_k::beam_reorder(h, h, row, row, L, layer, b.parents, groups, beams, err, s));
+  return RNET_OK;
+}
+
+int Engine::beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha, int* d_sequences,
+                        int* d_lengths, float* d_scores, bool use_graph) {
+  if (d->M % beams)
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: n_streams must be a multiple of beams");
+  if (d->M / beams > 65535)
+    return rnet_status::fail(RNET_ERR_UNSUPPORTED, "beam_search: more than 65535 sequences");
+  int rc = beam_reserve(d, n_steps);
+  if (rc) return rc;
+  Decoder::Beam& b = d->beam;
+  const int groups = d->M / beams;
+  cudaStream_t s = stream_;
+  if (b.exec && (b.beams != beams || b.eos != eos)) {
+    cudaGraphExecDestroy(b.exec);
+    b.exec = nullptr;
+  }
+  auto step = [&]() {
+    const int r = beam_choose(d, beams, eos);
+    return r ? r : decode_logits(d);
+  };
+  CK(rnet_k::beam_begin(b.scores, b.finished, b.step, groups, beams, s));
+  for (int i = 0; i + 1 < n_steps; ++i) {
+    // the first step is eager: kernel attributes and tensor maps are set up
+    // outside the capture
+    if (use_graph && i > 0 && !b.exec) {
+      CK(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal));
+      rc = step();
+      cudaGraph_t g = nullptr;
+      const cudaError_t ce = cudaStreamEndCapture(s, &g);
+      size_t nodes = 0;
+      cudaError_t ge = ce;
+      if (rc == RNET_OK && ge == cudaSuccess) ge = cudaGraphGetNodes(g, nullptr, &nodes);
+      if (rc == RNET_OK && ge == cudaSuccess) ge = cudaGraphInstantiate(&b.exec, g, 0);
+      if (g) cudaGraphDestroy(g);
+      if (rc) return rc;
+      if (ge != cudaSuccess) b.exec = nullptr;
+      CK(ge);
+      b.kernels = (int)nodes;  // kernel nodes only
+      b.beams = beams;
+      b.eos = eos;
+    }
+    if (use_graph && b.exec) {
+      CK(cudaGraphLaunch(b.exec, s));
+      rnet_status::count_launch((unsigned)b.kernels);
+    } else {
+      rc = step();
+      if (rc) return rc;
+    }
+  }
+  rc = beam_choose(d, beams, eos);
+  if (rc) return rc;
+  CK(rnet_k::beam_backtrack(b.hist_tokens, b.hist_parents, b.scores, eos, alpha, d_sequences,
+                            d_lengths, d_scores, n_steps, groups, beams,
+                            rnet_status::device_error_word(), s));
   return RNET_OK;
 }
 

@@ -93,6 +93,18 @@ struct Decoder {
   float temperature = 0.0f;
   float top_p = 1.0f;
   unsigned long long seed = 0;
+  // beam search: per stream the score, whether it has ended and its parent of
+  // the last selection; the selections' tokens and parents, row by row
+  struct Beam {
+    float* scores = nullptr;
+    int *finished = nullptr, *parents = nullptr, *step = nullptr;
+    void* arena = nullptr;
+    int *hist_tokens = nullptr, *hist_parents = nullptr;  // [cap, M]
+    int cap = 0;
+    // the captured step and what it holds
+    cudaGraphExec_t exec = nullptr;
+    int beams = 0, eos = 0, kernels = 0;
+  } beam;
 };
 
 class Engine {
@@ -102,12 +114,19 @@ class Engine {
   void decoder_free(Decoder* d);
   // Chunked-scan forward over d_tokens [M, T]; leaves the state after T
   // tokens, last-position logits in d->logits and their argmax in d->tok.
-  int prefill(Decoder* d, const int* d_tokens, int T);
+  // With copies > 1 d_tokens is [M / copies, T] and `copies` streams in a row
+  // start from each prompt.
+  int prefill(Decoder* d, const int* d_tokens, int T, int copies = 1);
   // One token per stream (d_tokens, or the previous argmax when null);
   // logits in d->logits, argmax in d->tok.
   int decode_step(Decoder* d, const int* d_tokens);
   // n_steps greedy steps; d_out [n_steps][M] receives the generated tokens.
   int generate(Decoder* d, int n_steps, int* d_out, bool use_graph);
+  // Beam search of n_steps tokens from the state and logits at hand (after a
+  // prefill): groups of `beams` streams are the beams of one sequence, all
+  // starting from the first stream of the group. Outputs as rnet_beam_backtrack.
+  int beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha, int* d_sequences,
+                  int* d_lengths, float* d_scores, bool use_graph);
 
   explicit Engine(const rnet_model_config& c);
   ~Engine();
@@ -138,6 +157,13 @@ class Engine {
   // the step's launches in order (what the graph captures)
   int train_step_eager(const int* d_in, const int* d_tgt, int B, int T, float lr, float clip,
                        float* d_loss_sum);
+
+  // The step with rnet_distill_topk_forward's loss in the place of the
+  // cross-entropy (dlogits scaled by 1/N); always eager.
+  int train_step_distill(const int* d_in, const int* t_idx, const float* t_val,
+                         const float* t_lse, const int* d_tgt, const float* row_weight, int B,
+                         int T, int top_k, float tau, float soft, float hard, float lr, float clip,
+                         float* d_loss_sum);
 
   // Optimizer extensions (off by default: the reference's plain SGD with
   // clipping, src/resonance_net.cpp:551-663): momentum, weight decay added
@@ -198,6 +224,12 @@ class Engine {
   void prof_end(cudaEvent_t a, int kind, double flops, double bytes);
 
   int gemm_err(cudaError_t e, const char* what);
+  // the decode step up to the logits, for the tokens in d->tok
+  int decode_logits(Decoder* d);
+  int beam_reserve(Decoder* d, int n_steps);
+  // one selection: tokens, parents and scores from the logits, recorded, and the
+  // states in the order of the parents
+  int beam_choose(Decoder* d, int beams, int eos);
   // train: keep the activation caches the backward reads (scan keeps e = h~ -
   // h_prev in LayerAct::h); otherwise LayerAct::h holds h (prefill)
   int layer_forward(int l, const float* Xl, float* Xn, LayerAct& a, int B, int T, bool train);
@@ -267,6 +299,8 @@ class Engine {
   int* g_tgt_ = nullptr;
   int g_cap_ = 0;
   float* velocity_ = nullptr;
+  float* row_loss_ = nullptr;  // distillation: a loss per token
+  int row_loss_cap_ = 0;
   // asynchronous save
   float* snap_ = nullptr;   // device snapshot of params_
   float* snap_host_ = nullptr;  // pinned

@@ -144,9 +144,12 @@ cudaError_t fold_rows(const float* A, const float* B, size_t bd, size_t bj, floa
 cudaError_t decode_conv(const float* n, float* ring, const int* pos, const float* w3,
                         const float* w7, const float* w15, float* S, int M, int D,
                         cudaStream_t s);
+// copies: streams m * copies .. m * copies + copies - 1 start from row m of the
+// prefill (M streams in all).
 cudaError_t decode_extract_state(const float* n1, const float* h, float* ring, float* hs, int M,
-                                 int T, int D, cudaStream_t s);
-cudaError_t last_rows(const float* x, float* out, int M, int T, int D, cudaStream_t s);
+                                 int T, int D, cudaStream_t s, int copies = 1);
+cudaError_t last_rows(const float* x, float* out, int M, int T, int D, cudaStream_t s,
+                      int copies = 1);
 cudaError_t argmax_rows(const float* logits, int M, int V, int* tok, int* out, int* pos,
                         cudaStream_t s);
 // Next token per row: greedy (temperature <= 0, as argmax_rows) or
@@ -187,6 +190,13 @@ cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float
 cudaError_t beam_reorder(const void* src, void* dst, size_t row_bytes, size_t pitch, size_t outer,
                          size_t outer_pitch, const int* parents, int batch, int beams,
                          unsigned* err, cudaStream_t s);
+// A search begins: scores {0, -inf, ...} per sequence, finished 0, *step 0.
+cudaError_t beam_begin(float* scores, int* finished, int* step, int batch, int beams,
+                       cudaStream_t s);
+// Row *step of the histories [.., M] = tokens / parents; then *step += 1, and
+// *pos += 1 unless this was the first row (the step before it fed a token).
+cudaError_t beam_record(const int* tokens, const int* parents, int* hist_tokens,
+                        int* hist_parents, int M, int* step, int* pos, cudaStream_t s);
 // Follows the recorded parents [steps, batch * beams] back from the last step;
 // sequences [batch * beams, steps] ranked by score / length^alpha.
 cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
