@@ -135,15 +135,21 @@ __device__ __forceinline__ void store_u32(uint32_t ra, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ra), "r"(v) : "memory");
 }
 
+// Two CTAs of 512 threads to an SM hide each other's latency better than more
+// values to a thread (32 x 8 rows of 50001 fp32: 24.7 us with 256 threads of 32
+// values, XX us so).
+template <class T>
+using BeamSelection = Selection<T, 512, 16>;
+
 // Longer rows: a cluster per sequence. The W * S (beam, slice) parts go round the
 // CTAs of the cluster; their lists meet in the first CTA's shared memory.
 template <class T>
-__global__ void __launch_bounds__(SEL_THREADS) beam_select_cluster_kernel(
+__global__ void __launch_bounds__(BeamSelection<T>::NT, 2) beam_select_cluster_kernel(
     const T* __restrict__ logits, long long ld, SelectArgs a, int S, int slice) {
   rnet_dev::pdl_trigger();
   __shared__ Lists lists;
   extern __shared__ uint4 cluster_buf[];
-  Selection<T>& sel = *reinterpret_cast<Selection<T>*>(cluster_buf);
+  auto& sel = *reinterpret_cast<BeamSelection<T>*>(cluster_buf);
   const int tid = threadIdx.x, rank = blockIdx.y, C = gridDim.y;
   const size_t m0 = (size_t)blockIdx.x * a.W;
   // the first CTA's shared memory may be written once it runs
@@ -193,17 +199,17 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
   }
   // slices of a row where the rows alone leave SMs idle, one pass or more each
   int S = 1;
-  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * Selection<T>::CHUNK * N < a.V) ++S;
+  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * BeamSelection<T>::CHUNK * N < a.V) ++S;
   const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
   const int C = a.W * S < 8 ? a.W * S : 8;
   auto kernel = beam_select_cluster_kernel<T>;
   static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem((const void*)kernel, sizeof(Selection<T>), ready);
+  cudaError_t e = allow_smem((const void*)kernel, sizeof(BeamSelection<T>), ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch, C);
-  cfg.blockDim = dim3(SEL_THREADS);
-  cfg.dynamicSmemBytes = sizeof(Selection<T>);
+  cfg.blockDim = dim3(BeamSelection<T>::NT);
+  cfg.dynamicSmemBytes = sizeof(BeamSelection<T>);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -52,13 +52,16 @@ __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __r
   if (lane == 0 && a.lse) a.lse[row] = log_sum(m, s, a.inv_tau);
 }
 
+template <class T>
+using TopkSelection = Selection<T, 256, 32>;
+
 // Longer rows: a CTA per row.
 template <class T>
-__global__ void __launch_bounds__(SEL_THREADS, sizeof(T) == 2 ? 4 : 2) topk_cta_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(TopkSelection<T>::NT, sizeof(T) == 2 ? 4 : 2) topk_cta_kernel(const T* __restrict__ logits,
                                                                long long ld, TopkArgs a) {
   rnet_dev::pdl_trigger();
   extern __shared__ uint4 sel_buf[];
-  Selection<T>& sel = *reinterpret_cast<Selection<T>*>(sel_buf);
+  auto& sel = *reinterpret_cast<TopkSelection<T>*>(sel_buf);
   const size_t row = blockIdx.x;
   float m;
   double s;
@@ -81,9 +84,9 @@ cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, c
   else {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e =
-        allow_smem((const void*)topk_cta_kernel<T>, sizeof(Selection<T>), ready);
+        allow_smem((const void*)topk_cta_kernel<T>, sizeof(TopkSelection<T>), ready);
     if (e != cudaSuccess) return e;
-    topk_cta_kernel<T><<<rows, SEL_THREADS, sizeof(Selection<T>), s>>>(z, ld, a);
+    topk_cta_kernel<T><<<rows, TopkSelection<T>::NT, sizeof(TopkSelection<T>), s>>>(z, ld, a);
   }
   return cudaGetLastError();
 }

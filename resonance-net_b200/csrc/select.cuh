@@ -205,31 +205,33 @@ __device__ __forceinline__ int warp_select(const uint32_t* w, int K, float c, ui
 }
 
 // ---------------------------------------------------------------- a CTA
-constexpr int SEL_THREADS = 256;
-constexpr int SEL_WARPS = SEL_THREADS / 32;
-constexpr int SEL_GROUP = 4;          // words that are kept together
-constexpr int SEL_STAGES = 2;         // chunks in shared memory
-constexpr int SEL_QUEUE = 512;        // groups kept at most
-constexpr int SEL_CAP = 512;          // keys kept at most
+constexpr int SEL_GROUP = 4;    // words that are kept together
+constexpr int SEL_STAGES = 2;   // chunks in shared memory
+constexpr int SEL_QUEUE = 512;  // groups kept at most
+constexpr int SEL_CAP = 512;    // keys kept at most
 
-template <class T>
+// The shared memory of a CTA of NT threads that take VALUES values each of one
+// chunk.
+template <class T, int NT_, int VALUES>
 struct alignas(16) Selection {
+  using Type = T;
+  static constexpr int NT = NT_, WARPS = NT / 32;
   static constexpr int N = Words<T>::N;
-  static constexpr int R = 32 / N;             // words of a thread in one chunk
-  static constexpr int CHUNK = SEL_THREADS * R;  // words
+  static constexpr int R = VALUES / N;   // words of a thread in one chunk
+  static constexpr int CHUNK = NT * R;   // words
   uint32_t ring[SEL_STAGES][CHUNK + 4];
   uint32_t group[SEL_GROUP][SEL_QUEUE];
   int group_word[SEL_QUEUE];  // the group's first word
   uint64_t key[SEL_CAP];
-  double s[SEL_WARPS];
-  float bound[2][SEL_WARPS], m[SEL_WARPS];
+  double s[WARPS];
+  float bound[2][WARPS], m[WARPS];
   uint64_t bar[SEL_STAGES];
   int keys, groups, abort[2];
 };
 
 // Once per CTA, before the first selection; parity belongs to the barriers.
-template <class T>
-__device__ __forceinline__ void select_setup(Selection<T>& sel, uint32_t& parity) {
+template <class Sel>
+__device__ __forceinline__ void select_setup(Sel& sel, uint32_t& parity) {
   parity = 0;
   if (threadIdx.x == 0) {
     sel.abort[0] = sel.abort[1] = 0;
@@ -241,13 +243,13 @@ __device__ __forceinline__ void select_setup(Selection<T>& sel, uint32_t& parity
 // Leaves the K largest of the n <= SEL_CAP keys, or those of them that `keep`
 // accepts, in any order, and returns a bound that exactly K of all n reach (0 if
 // there are no more than K). All threads, which have read n before.
-template <class T, class Keep>
-__device__ __forceinline__ uint64_t shrink(Selection<T>& sel, int n, int K, Keep keep) {
-  constexpr int J = SEL_CAP / SEL_THREADS;
+template <class Sel, class Keep>
+__device__ __forceinline__ uint64_t shrink(Sel& sel, int n, int K, Keep keep) {
+  constexpr int NT = Sel::NT, J = (SEL_CAP + NT - 1) / NT;
   uint64_t k[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int i = threadIdx.x + j * SEL_THREADS;
+    const int i = threadIdx.x + j * NT;
     k[j] = i < n ? sel.key[i] : 0;
   }
   uint64_t t = 0;
@@ -257,7 +259,7 @@ __device__ __forceinline__ uint64_t shrink(Selection<T>& sel, int n, int K, Keep
       int reach = 0;
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        if (j * SEL_THREADS < n) reach += __syncthreads_count(k[j] >= u);
+        if (j * NT < n) reach += __syncthreads_count(k[j] >= u);
       if (reach >= K) t = u;
       if (reach == K) break;
     }
@@ -275,11 +277,12 @@ __device__ __forceinline__ uint64_t shrink(Selection<T>& sel, int n, int K, Keep
 // have read n before. Where they are more than there is room for, the bound is
 // raised to the K-th of those at hand and the groups are gone through again; the
 // keys of earlier groups (elements before `first`) stay.
-template <class T, bool CLEAN>
-__device__ __forceinline__ void drain(Selection<T>& sel, int n, int K, int first, uint64_t& bound) {
-  constexpr int N = Words<T>::N;
+template <bool CLEAN, class Sel>
+__device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_t& bound) {
+  using T = typename Sel::Type;
+  constexpr int N = Sel::N, NT = Sel::NT;
   for (bool again = true; again;) {
-    for (int i = threadIdx.x; i < n; i += SEL_THREADS) {
+    for (int i = threadIdx.x; i < n; i += NT) {
       const int word = sel.group_word[i];
 #pragma unroll
       for (int j = 0; j < SEL_GROUP; ++j)
@@ -287,7 +290,7 @@ __device__ __forceinline__ void drain(Selection<T>& sel, int n, int K, int first
         for (int h = 0; h < N; ++h) {
           const float x = word_value<T, CLEAN>(sel.group[j][i], h);
           if (!(x > -INFINITY)) continue;
-          const uint64_t k = make_key(x + 0.0f, (word + j * SEL_THREADS) * N + h);
+          const uint64_t k = make_key(x + 0.0f, (word + j * NT) * N + h);
           if (k < bound) continue;
           const int at = atomicAdd(&sel.keys, 1);
           if (at < SEL_CAP) sel.key[at] = k;
@@ -308,13 +311,13 @@ __device__ __forceinline__ void drain(Selection<T>& sel, int n, int K, int first
 
 // The K <= 64 largest of the elements [begin, end) of the row z (begin on a
 // 16-byte place of the row, and a multiple of 2). sel.key[0 .. return value) are
-// sorted. m is the slice's largest logit, s the sum. All SEL_THREADS threads; sel
+// sorted. m is the slice's largest logit, s the sum. All threads; sel
 // is set up and not in use.
-template <class T, bool CLEAN>
-__device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int begin, int end, int K,
+template <bool CLEAN, class Sel, class T>
+__device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, int end, int K,
                                              float c, float& m, double& s, uint32_t& parity,
                                              unsigned* err) {
-  constexpr int N = Words<T>::N, R = Selection<T>::R, CHUNK = Selection<T>::CHUNK;
+  constexpr int N = Sel::N, R = Sel::R, CHUNK = Sel::CHUNK, NT = Sel::NT, WARPS = Sel::WARPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool even = even_start(z);
   const int total = begin < end ? (end - begin + N - 1) / N : 0;  // words
@@ -360,19 +363,19 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
       if (even) {
 #pragma unroll
         for (int j = 0; j < R; ++j)
-          w[j] = *reinterpret_cast<const uint32_t*>(p + 4 * SEL_THREADS * j);
+          w[j] = *reinterpret_cast<const uint32_t*>(p + 4 * NT * j);
       } else {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
           const unsigned short* q =
-              reinterpret_cast<const unsigned short*>(p + 4 * SEL_THREADS * j);
+              reinterpret_cast<const unsigned short*>(p + 4 * NT * j);
           w[j] = q[0] | (uint32_t)q[1] << 16;
         }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < R; ++j)
-        w[j] = load_word(z, w0 + j * SEL_THREADS + tid, end, even);
+        w[j] = load_word(z, w0 + j * NT + tid, end, even);
     }
     float top[R / SEL_GROUP];
     float mine = -INFINITY;
@@ -386,12 +389,12 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
     m = mx;
     if (i < 4 || (i & 3) == 0) {
       // K logits reach the least of the warps' r-th largest thread maxima so far
-      const float v = K <= SEL_WARPS ? warp_max(m) : warp_nth(m, (K + SEL_WARPS - 1) / SEL_WARPS);
+      const float v = K <= WARPS ? warp_max(m) : warp_nth(m, (K + WARPS - 1) / WARPS);
       if (lane == 0) sel.bound[i & 1][warp] = v;
       __syncthreads();
       float least = sel.bound[i & 1][0];
 #pragma unroll
-      for (int j = 1; j < SEL_WARPS; ++j) least = fminf(least, sel.bound[i & 1][j]);
+      for (int j = 1; j < WARPS; ++j) least = fminf(least, sel.bound[i & 1][j]);
       const uint64_t t = (uint64_t)order(least + 0.0f) << 32;
       if (t > bound) {
         bound = t;
@@ -411,7 +414,7 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
 #pragma unroll
         for (int h = 0; h < N; ++h)
           in |= make_key(word_value<T, CLEAN>(v, h) + 0.0f,
-                         (w0 + (g * SEL_GROUP + j) * SEL_THREADS + tid) * N + h) >= bound;
+                         (w0 + (g * SEL_GROUP + j) * NT + tid) * N + h) >= bound;
       }
       return in;
     };
@@ -423,7 +426,7 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
           const int at = atomicAdd(&sel.groups, 1);
           full |= at >= SEL_QUEUE - SEL_QUEUE / 4;
           if (at < SEL_QUEUE) {
-            sel.group_word[at] = w0 + g * SEL_GROUP * SEL_THREADS + tid;
+            sel.group_word[at] = w0 + g * SEL_GROUP * NT + tid;
 #pragma unroll
             for (int j = 0; j < SEL_GROUP; ++j) sel.group[j][at] = w[g * SEL_GROUP + j];
           }
@@ -438,7 +441,7 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
         const int n = sel.groups;
         __syncthreads();
         again = n > SEL_QUEUE;  // then this chunk's groups come again
-        drain<T, CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound);
+        drain<CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound);
         const int got = sel.keys, here = w0 * N;
         __syncthreads();
         const uint64_t t = shrink(sel, got, K, [&](uint64_t k) {
@@ -459,11 +462,11 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
   {
     const int n = sel.groups;
     __syncthreads();
-    drain<T, CLEAN>(sel, n, K, epoch, bound);
+    drain<CLEAN>(sel, n, K, epoch, bound);
   }
   int n = sel.keys;
   __syncthreads();
-  if (n > SEL_THREADS) {
+  if (n > NT) {
     shrink(sel, n, K, [](uint64_t) { return true; });
     n = sel.keys;
   }
@@ -478,23 +481,23 @@ __device__ __forceinline__ int cta_select_as(Selection<T>& sel, const T* z, int 
   const float mine = m;
   m = sel.m[0];
 #pragma unroll
-  for (int i = 1; i < SEL_WARPS; ++i) m = fmaxf(m, sel.m[i]);
+  for (int i = 1; i < WARPS; ++i) m = fmaxf(m, sel.m[i]);
   const double part = warp_sum((double)(sum * exp2_fast((mine - m) * c)));
   if (lane == 0) sel.s[warp] = part;
   __syncthreads();
   s = 0.0;
 #pragma unroll
-  for (int i = 0; i < SEL_WARPS; ++i) s += sel.s[i];
+  for (int i = 0; i < WARPS; ++i) s += sel.s[i];
   return min(n, K);
 }
-template <class T>
-__device__ __forceinline__ int cta_select(Selection<T>& sel, const T* z, int begin, int end, int K,
+template <class Sel, class T>
+__device__ __forceinline__ int cta_select(Sel& sel, const T* z, int begin, int end, int K,
                                           float c, float& m, double& s, uint32_t& parity,
                                           unsigned* err) {
-  int n = cta_select_as<T, false>(sel, z, begin, end, K, c, m, s, parity, err);
+  int n = cta_select_as<false>(sel, z, begin, end, K, c, m, s, parity, err);
   if (s != s) {
     __syncthreads();
-    n = cta_select_as<T, true>(sel, z, begin, end, K, c, m, s, parity, err);
+    n = cta_select_as<true>(sel, z, begin, end, K, c, m, s, parity, err);
   }
   return n;
 }
