@@ -31,7 +31,8 @@ __device__ __forceinline__ void write_place(const TopkArgs& a, size_t row, int k
 
 constexpr int TOPK_WARPS = 4;
 
-// Rows of up to 32 * R words: a warp per row.
+// Rows of up to 32 * R words: a warp per row. 64 values a lane spill a little and
+// are still the faster way (4096 rows of 2000 fp32: 18.4 us, 29.9 with a CTA a row).
 template <class T, int R>
 __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __restrict__ logits,
                                                                     long long ld, TopkArgs a,
@@ -52,16 +53,13 @@ __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __r
   if (lane == 0 && a.lse) a.lse[row] = log_sum(m, s, a.inv_tau);
 }
 
-template <class T>
-using TopkSelection = Selection<T, 256, 32>;
-
-// Longer rows: a CTA per row.
-template <class T>
-__global__ void __launch_bounds__(TopkSelection<T>::NT, sizeof(T) == 2 ? 4 : 2) topk_cta_kernel(const T* __restrict__ logits,
-                                                               long long ld, TopkArgs a) {
+// Longer rows: a CTA of NT threads per row.
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, NT > 128 ? 1 : sizeof(T) == 2 ? 7 : 4)
+    topk_cta_kernel(const T* __restrict__ logits, long long ld, TopkArgs a) {
   rnet_dev::pdl_trigger();
   extern __shared__ uint4 sel_buf[];
-  auto& sel = *reinterpret_cast<TopkSelection<T>*>(sel_buf);
+  auto& sel = *reinterpret_cast<Selection<T, NT, 32>*>(sel_buf);
   const size_t row = blockIdx.x;
   float m;
   double s;
@@ -73,6 +71,17 @@ __global__ void __launch_bounds__(TopkSelection<T>::NT, sizeof(T) == 2 ? 4 : 2) 
   if (threadIdx.x == 0 && a.lse) a.lse[row] = log_sum(m, (float)s, a.inv_tau);
 }
 
+template <class T, int NT>
+cudaError_t topk_cta(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
+  auto kernel = topk_cta_kernel<T, NT>;
+  constexpr int smem = sizeof(Selection<T, NT, 32>);
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = allow_smem((const void*)kernel, smem, ready);
+  if (e != cudaSuccess) return e;
+  kernel<<<rows, NT, smem, s>>>(z, ld, a);
+  return cudaGetLastError();
+}
+
 template <class T>
 cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
   constexpr int N = Words<T>::N;
@@ -81,13 +90,13 @@ cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, c
     topk_warp_kernel<T, 8 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
   else if (a.V <= 1024)
     topk_warp_kernel<T, 32 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
-  else {
-    static std::atomic<uint64_t> ready{0};
-    const cudaError_t e =
-        allow_smem((const void*)topk_cta_kernel<T>, sizeof(TopkSelection<T>), ready);
-    if (e != cudaSuccess) return e;
-    topk_cta_kernel<T><<<rows, TopkSelection<T>::NT, sizeof(TopkSelection<T>), s>>>(z, ld, a);
-  }
+  else if (a.V <= 2048)
+    topk_warp_kernel<T, 64 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
+  else
+    // while every row has an SM of its own, more threads for it (148 rows of 50001
+    // fp32, top 64: 16.0 us with 512 threads, 26.9 with 128; 592 rows: 35.7 with 128;
+    // 256 threads lie between)
+    return rows <= 148 ? topk_cta<T, 512>(z, ld, a, rows, s) : topk_cta<T, 128>(z, ld, a, rows, s);
   return cudaGetLastError();
 }
 

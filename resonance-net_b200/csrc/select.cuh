@@ -130,15 +130,26 @@ __device__ __forceinline__ int warp_select_as(const uint32_t* w, int K, float c,
   m = fmaxf(warp_max(mine), -FLT_MAX);
   s = warp_sum((Sum)words_sum<T, R, CLEAN>(w, m, c));
   if (!CLEAN && s != s) return 0;
-  // K logits reach T: from K lanes, or two each from K / 2 lanes
+  // K logits reach T: the K-th largest of the lanes' maxima, or, where that would be
+  // a small one, about the K-th largest of the maxima of the lanes' quarters
   float T_;
-  if (K <= 32 || R == 1) {
-    T_ = K <= 32 ? warp_nth(mine, K) : -INFINITY;
+  if (K <= 16) {
+    T_ = warp_nth(mine, K);
   } else {
-    constexpr int H = (R + 1) / 2;
-    T_ = warp_nth(fminf(words_max<T, H, CLEAN>(w),
-                        words_max<T, R - H ? R - H : 1, CLEAN>(w + H % R)),
-                  (K + 1) / 2);
+    constexpr int Q = R / 4;
+    uint32_t g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = order(words_max<T, Q, CLEAN>(w + i * Q) + 0.0f);
+    uint32_t o = 0;
+    for (uint32_t b = 1u << 31; b > 1u << 12; b >>= 1) {
+      int k = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k += g[i] >= (o | b);
+      k = __reduce_add_sync(~0u, k);
+      if (k >= K) o |= b;
+      if (k >= K && k <= K + K / 8) break;
+    }
+    T_ = o > order(-FLT_MAX) ? unorder(o) : -FLT_MAX;
   }
   T_ = fmaxf(T_, -FLT_MAX);  // -inf is no candidate
   int mine_in = 0;
@@ -162,13 +173,19 @@ __device__ __forceinline__ int warp_select_as(const uint32_t* w, int K, float c,
       each([&](float x, int e) { k += x > -INFINITY && f(order(x + 0.0f), (uint32_t)e); });
       return __reduce_add_sync(~0u, k);
     };
-    uint32_t o = 0, last = 0;
-    for (uint32_t b = 1u << 31; b; b >>= 1)
-      if (reach([&](uint32_t x, uint32_t) { return x >= (o | b); }) >= K) o |= b;
-    const int above = reach([&](uint32_t x, uint32_t) { return x > o; });
-    for (uint32_t b = 1u << 10; b; b >>= 1)
-      if (reach([&](uint32_t x, uint32_t e) { return x == o && e < (last | b); }) < K - above)
-        last |= b;
+    uint32_t o = 0, last = ~0u;
+    int got = 0;
+    for (uint32_t b = 1u << 31; b && got != K; b >>= 1) {
+      const int k = reach([&](uint32_t x, uint32_t) { return x >= (o | b); });
+      if (k >= K) o |= b, got = k;
+    }
+    if (got != K) {
+      const int above = reach([&](uint32_t x, uint32_t) { return x > o; });
+      last = 0;
+      for (uint32_t b = 1u << 11; b; b >>= 1)
+        if (reach([&](uint32_t x, uint32_t e) { return x == o && e < (last | b); }) < K - above)
+          last |= b;
+    }
     n = 0;
     each([&](float x, int e) {
       const uint32_t v = order(x + 0.0f);
@@ -387,7 +404,7 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
     const float mx = fmaxf(m, mine);
     sum = sum * exp2_fast((m - mx) * c) + words_sum<T, R, CLEAN>(w, mx, c);
     m = mx;
-    if (i < 4 || (i & 3) == 0) {
+    if (i < 2 || (i & (i - 1)) == 0) {
       // K logits reach the least of the warps' r-th largest thread maxima so far
       const float v = K <= WARPS ? warp_max(m) : warp_nth(m, (K + WARPS - 1) / WARPS);
       if (lane == 0) sel.bound[i & 1][warp] = v;
