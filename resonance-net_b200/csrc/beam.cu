@@ -99,30 +99,6 @@ __device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size
   }
 }
 
-// Rows of up to 32 * R words: a CTA per sequence, a warp per beam.
-template <class T, int R, int MOST>
-__global__ void __launch_bounds__(32 * MOST) beam_select_warps_kernel(
-    const T* __restrict__ logits, long long ld, SelectArgs a) {
-  rnet_dev::pdl_trigger();
-  __shared__ Lists lists;
-  extern __shared__ uint64_t keys[];  // WARP_CAP a warp
-  const int lane = threadIdx.x & 31, beam = threadIdx.x >> 5;
-  const size_t m0 = (size_t)blockIdx.x * a.W;
-  const T* z = logits + (m0 + beam) * ld;
-  const bool even = even_start(z);
-  uint32_t w[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) w[j] = load_word(z, lane + 32 * j, a.V, even);
-  uint64_t* own = keys + beam * WARP_CAP;
-  float m;
-  double s;
-  const int n = warp_select<T, R>(w, a.W, LOG2E, own, m, s);
-  if (lane < n) lists.key[beam][lane] = own[lane];
-  if (lane == 0) lists.n[beam] = n, lists.m[beam] = m, lists.s[beam] = s;
-  __syncthreads();
-  if (beam == 0) merge(lists, a, m0, 1);
-}
-
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
   uint32_t ra;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(ra) : "r"(rnet_dev::smem_u32(p)));
@@ -135,9 +111,57 @@ __device__ __forceinline__ void store_u32(uint32_t ra, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ra), "r"(v) : "memory");
 }
 
+// A part's list and sum, into the first CTA's shared memory: lane (or thread) t
+// brings key t.
+__device__ __forceinline__ void deliver(Lists& lists, int u, int t, int n, uint64_t key, float m,
+                                        double s) {
+  if (t < n) store_u64(in_first_cta(&lists.key[u][t]), key);
+  if (t == 0) {
+    store_u32(in_first_cta(&lists.n[u]), n);
+    store_u32(in_first_cta(&lists.m[u]), __float_as_uint(m));
+    store_u64(in_first_cta(&lists.s[u]), (uint64_t)__double_as_longlong(s));
+  }
+}
+
+constexpr int ROWS = 8;  // beams of a CTA of the warp-per-beam kernel
+
+// Rows of up to 32 * R words: a warp per beam, eight beams to a CTA, a cluster of
+// CTAs per sequence.
+template <class T, int R>
+__global__ void __launch_bounds__(32 * ROWS) beam_select_warps_kernel(
+    const T* __restrict__ logits, long long ld, SelectArgs a) {
+  rnet_dev::pdl_trigger();
+  __shared__ Lists lists;
+  __shared__ uint64_t keys[ROWS][WARP_CAP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int beam = blockIdx.y * ROWS + warp;
+  const size_t m0 = (size_t)blockIdx.x * a.W;
+  // the first CTA's shared memory may be written once it runs
+  const bool many = gridDim.y > 1;
+  if (many) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  float m = 0.f;
+  double s = 0.0;
+  int n = 0;
+  if (beam < a.W) {
+    const T* z = logits + (m0 + beam) * ld;
+    const bool even = even_start(z);
+    uint32_t w[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) w[j] = load_word(z, lane + 32 * j, a.V, even);
+    n = warp_select<T, R>(w, a.W, LOG2E, keys[warp], m, s);
+  }
+  if (many) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (beam < a.W) deliver(lists, beam, lane, n, keys[warp][lane], m, s);
+  if (many) rnet_dev::cluster_sync();
+  else __syncthreads();
+  if (blockIdx.y == 0 && warp == 0) merge(lists, a, m0, 1);
+}
+
+constexpr int SELECT_CTAS = 16;  // of one sequence's cluster
+
 // Two CTAs of 512 threads to an SM hide each other's latency better than more
 // values to a thread (32 x 8 rows of 50001 fp32: 24.7 us with 256 threads of 32
-// values, XX us so).
+// values, 23.3 us so).
 template <class T>
 using BeamSelection = Selection<T, 512, 16>;
 
@@ -167,49 +191,20 @@ __global__ void __launch_bounds__(BeamSelection<T>::NT, 2) beam_select_cluster_k
                      parity, a.err);
     if (!waited) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     waited = true;
-    if (tid < n) store_u64(in_first_cta(&lists.key[u][tid]), sel.key[tid]);
-    if (tid == 0) {
-      store_u32(in_first_cta(&lists.n[u]), n);
-      store_u32(in_first_cta(&lists.m[u]), __float_as_uint(m));
-      store_u64(in_first_cta(&lists.s[u]), (uint64_t)__double_as_longlong(s));
-    }
+    deliver(lists, u, tid, n, tid < n ? sel.key[tid] : 0, m, s);
     __syncthreads();  // sel is free again
   }
   if (C > 1) rnet_dev::cluster_sync();
   if (rank == 0 && tid < 32) merge(lists, a, m0, S);
 }
 
-template <class T>
-cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int batch,
-                          cudaStream_t s) {
-  constexpr int N = Words<T>::N;
-  const int block = 32 * a.W;
-  const size_t smem = (size_t)a.W * WARP_CAP * sizeof(uint64_t);
-  if (a.V <= 256 && a.W <= 8) {
-    beam_select_warps_kernel<T, 8 / N, 8><<<batch, block, smem, s>>>(z, ld, a);
-    return cudaGetLastError();
-  }
-  if (a.V <= 256) {
-    beam_select_warps_kernel<T, 8 / N, 32><<<batch, block, smem, s>>>(z, ld, a);
-    return cudaGetLastError();
-  }
-  if (a.V <= 1024 && a.W <= 8) {  // more beams leave a thread too few registers for the row
-    beam_select_warps_kernel<T, 32 / N, 8><<<batch, block, smem, s>>>(z, ld, a);
-    return cudaGetLastError();
-  }
-  // slices of a row where the rows alone leave SMs idle, one pass or more each
-  int S = 1;
-  while (a.W * (S + 1) <= 8 && (long long)batch * a.W * (S + 1) <= 2 * 148 && S * BeamSelection<T>::CHUNK * N < a.V) ++S;
-  const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
-  const int C = a.W * S < 8 ? a.W * S : 8;
-  auto kernel = beam_select_cluster_kernel<T>;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem((const void*)kernel, sizeof(BeamSelection<T>), ready);
-  if (e != cudaSuccess) return e;
+template <class Kernel, class... Args>
+cudaError_t launch_cluster(Kernel kernel, int batch, int C, int threads, size_t smem,
+                           cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch, C);
-  cfg.blockDim = dim3(BeamSelection<T>::NT);
-  cfg.dynamicSmemBytes = sizeof(BeamSelection<T>);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -217,7 +212,33 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
   at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, kernel, z, ld, a, S, slice);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <class T>
+cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int batch,
+                          cudaStream_t s) {
+  constexpr int N = Words<T>::N;
+  if (a.V <= 2048) {
+    const int C = (a.W + ROWS - 1) / ROWS, threads = 32 * (a.W < ROWS ? a.W : ROWS);
+    auto kernel = a.V <= 256    ? beam_select_warps_kernel<T, 8 / N>
+                  : a.V <= 1024 ? beam_select_warps_kernel<T, 32 / N>
+                                : beam_select_warps_kernel<T, 64 / N>;
+    return launch_cluster(kernel, batch, C, threads, 0, s, z, ld, a);
+  }
+  // slices of a row where the rows alone leave SMs idle, a chunk or more each
+  int S = 1;
+  while (a.W * (S + 1) <= SELECT_CTAS && (long long)batch * a.W * (S + 1) <= 148 &&
+         S * BeamSelection<T>::CHUNK * N < a.V)
+    ++S;
+  const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
+  const int C = a.W * S < SELECT_CTAS ? a.W * S : SELECT_CTAS;
+  auto kernel = beam_select_cluster_kernel<T>;
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem((const void*)kernel, sizeof(BeamSelection<T>), ready, true);
+  if (e != cudaSuccess) return e;
+  return launch_cluster(kernel, batch, C, BeamSelection<T>::NT, sizeof(BeamSelection<T>), s, z, ld,
+                        a, S, slice);
 }
 
 // ---------------------------------------------------------------- states

@@ -13,14 +13,18 @@
 
 namespace rnet_logits {
 
-// Lets a kernel use `bytes` of dynamic shared memory on the current device, once
-// per device: `ready` is the kernel's own record of devices.
-inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, and
+// clusters of more than 8 CTAs if it wants them, once per device: `ready` is the
+// kernel's own record of devices.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready,
+                              bool large_clusters = false) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 64 && (ready.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && large_clusters)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }
