@@ -134,8 +134,8 @@ struct RowGrad {
   }
 };
 
-// The record and label of one row, held by one warp: entry k in lane k % 32.
-template <int J>
+// The record and label of one row, held by G lanes: entry k in lane k % G.
+template <int J, int G>
 struct Record {
   int idx[J];  // -1: no entry
   float z[J], p[J], lp[J];  // student's logit, teacher's probability and its log
@@ -147,15 +147,21 @@ struct Record {
   // First the loads that depend on nothing, then the student's logits at the
   // indices.
   __device__ __forceinline__ void read(size_t row, const DistillArgs& a) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & (G - 1);
     y = a.hard != 0.f ? a.targets[row] : -1;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int k = lane + 32 * j;
+      const int k = lane + G * j;
       const bool in = k < a.K && a.soft != 0.f;
       idx[j] = in ? a.t_idx[row * a.K + k] : -1;
       lp[j] = in ? a.t_val[row * a.K + k] : -INFINITY;
     }
+  }
+  // No entry, no label.
+  __device__ __forceinline__ void clear() {
+    y = -1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) idx[j] = -1;
   }
   template <class T>
   __device__ __forceinline__ void gather(const T* row, int V) {
@@ -178,7 +184,7 @@ struct Record {
       tm = fmaxf(tm, lp[j]);
     }
     const bool given = a.t_lse != nullptr;
-    const float shift = given ? a.t_lse[row] : warp_max(tm);
+    const float shift = given ? a.t_lse[row] : group_max<G>(tm);
     float S = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -187,7 +193,7 @@ struct Record {
       p[j] = none ? 0.f : exp2_fast(lp[j] * LOG2E);
       S += p[j];
     }
-    P = warp_sum(S);
+    P = group_sum<G>(S);
     if (given || P == 0.f) return;
     const float inv = __fdividef(1.0f, P), ln = LN2 * log2_fast(P);
 #pragma unroll
@@ -218,13 +224,15 @@ struct Record {
   // once more with their own terms, after the stores of the whole share.
   template <bool HARD, class T, class In>
   __device__ __forceinline__ void fix(T* d, const RowGrad& g, int K, In in) const {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, base = lane & ~(G - 1);
     bool hot = false, twice = J > 1;
 #pragma unroll
     for (int j = 0; j < J; ++j) hot |= y >= 0 && idx[j] == y;
-    if (J == 1)
-      twice = __any_sync(~0u, (__match_any_sync(~0u, idx[0] < 0 ? ~lane : idx[0]) &
-                               ~(1u << lane)) != 0);
+    if (J == 1) {
+      // the same index in two lanes of a group (groups told apart by their first lane)
+      const int tag = idx[0] < 0 ? ~lane : idx[0] | base << 20;
+      twice = __any_sync(~0u, (__match_any_sync(~0u, tag) & ~(1u << lane)) != 0);
+    }
     float sum[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) sum[j] = p[j];
@@ -233,9 +241,9 @@ struct Record {
       for (int j = 0; j < J; ++j) sum[j] = 0.f;
 #pragma unroll
       for (int h = 0; h < J; ++h)
-        for (int k = 0; k < 32 && k + 32 * h < K; ++k) {
-          const int i = __shfl_sync(~0u, idx[h], k);
-          const float v = __shfl_sync(~0u, p[h], k);
+        for (int k = 0; k < G && k + G * h < K; ++k) {
+          const int i = __shfl_sync(~0u, idx[h], base + k);
+          const float v = __shfl_sync(~0u, p[h], base + k);
 #pragma unroll
           for (int j = 0; j < J; ++j)
             if (idx[j] == i) sum[j] += v;
@@ -248,8 +256,10 @@ struct Record {
         if (HARD && idx[j] == y) v -= g.hf;
         from_f(d + idx[j], v);
       }
-    if (HARD && !__any_sync(~0u, hot) && lane == 0 && y >= 0 && in(y))
-      from_f(d + y, g.at<HARD>(zy) - g.hf);
+    if (HARD) {
+      const uint32_t any = __ballot_sync(~0u, hot) >> base & (G == 32 ? ~0u : (1u << (G & 31)) - 1);
+      if (!any && lane == base && y >= 0 && in(y)) from_f(d + y, g.at<HARD>(zy) - g.hf);
+    }
   }
 };
 
@@ -344,47 +354,54 @@ __device__ __forceinline__ void zero_pieces(T* d, const Grid<T>& grid, int q0, i
 
 constexpr int WARPS = 8;  // rows of a CTA of the warp-per-row kernel
 
-// Rows of up to 32 * E elements in pieces: a warp per row.
-template <class T, int E, int J, bool HARD>
-__global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 4 : 2) distill_warp_kernel(
+// Rows of up to G * E elements in pieces: G lanes per row. With 16 lanes a warp
+// has two rows and what a row costs beside its elements is paid once for both.
+template <class T, int E, int G, int J, bool HARD>
+__global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) distill_warp_kernel(
     const T* logits, long long ld, T* dlogits, long long ldd, DistillArgs a, int rows) {
   rnet_dev::pdl_trigger();
-  constexpr int N = Piece<T>::N, NP = E / N;
-  const int lane = threadIdx.x & 31;
-  const size_t row = (size_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  constexpr int N = Piece<T>::N, NP = E / N, PER = 32 / G;
+  const int lane = threadIdx.x & (G - 1);
+  const size_t first = ((size_t)blockIdx.x * WARPS + (threadIdx.x >> 5)) * PER;
+  if (first >= rows) return;
+  // a group without a row of its own works on the last one, and keeps it to itself
+  const size_t own = first + (threadIdx.x & 31) / G;
+  const bool on = own < rows;
+  const size_t row = on ? own : rows - 1;
   const float w = a.weight ? a.weight[row] : 1.0f;
-  Record<J> r;
+  Record<J, G> r;
   r.read(row, a);
   const T* z = logits + row * ld;
   const Grid<T> grid(z, a.V);
   const int edge = grid.edge(lane);
   Piece<T> x[NP];
-  load_pieces<T, NP>(x, z, grid, lane, 32, grid.pieces);
-  const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
-  T* d = dlogits ? dlogits + row * ldd : nullptr;
-  if (w == 0.f) {  // whatever the row holds
-    if (d) zero_pieces(d, grid, lane, 32, grid.pieces, edge);
-    if (lane == 0) a.row_loss[row] = 0.f;
-    return;
+  load_pieces<T, NP>(x, z, grid, lane, G, grid.pieces);
+  float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
+  if (w == 0.f) {
+    // whatever the row holds: as one without a distribution, a record and a label
+#pragma unroll
+    for (int j = 0; j < NP; ++j) x[j].none();
+    xe = -INFINITY;
+    r.clear();
   }
   r.gather(z, a.V);
   const float c = a.inv_tau * LOG2E;
   Share<T, E, HARD> h;
   h.take(x, xe, c);
   r.weigh(row, a);
-  const float m = warp_max(h.m);
+  const float m = group_max<G>(h.m);
   const float f = rebase(h.m, m, c), f1 = HARD ? rebase(h.m, m, LOG2E) : 0.f;
-  const float s = warp_sum(h.s * f), s1 = HARD ? warp_sum(h.s1 * f1) : 0.f;
-  const float kl = warp_sum(r.kl(m, c));
-  if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
+  const float s = group_sum<G>(h.s * f), s1 = HARD ? group_sum<G>(h.s1 * f1) : 0.f;
+  const float kl = group_sum<G>(r.kl(m, c));
+  if (lane == 0 && on) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
-  if (!d) return;
+  if (!dlogits) return;
+  T* d = dlogits + row * ldd;
   const RowGrad g = row_factors(r.P, r.y >= 0, a, w, m, s, s1);
   __syncwarp();  // the reads of the row come before the stores, where dlogits are the logits
-  h.write(d, grid, lane, 32, grid.pieces, edge, g.a * f, g.a1 * f1);
+  if (on) h.write(d, grid, lane, G, grid.pieces, edge, g.a * f, g.a1 * f1);
   __syncwarp();  // orders the stores above before those below
-  r.template fix<HARD>(d, g, a.K, [](int) { return true; });
+  r.template fix<HARD>(d, g, a.K, [&](int) { return on; });
 }
 
 // A row's maximum and sums from the parts (m, s, s1) of n warps, joined in the
@@ -426,7 +443,7 @@ __global__ void __launch_bounds__(256) distill_cta_kernel(const T* logits, long 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row = blockIdx.x;
   const float w = a.weight ? a.weight[row] : 1.0f;
-  Record<J> r;
+  Record<J, 32> r;
   if (warp == 0) r.read(row, a);
   const T* z = logits + row * ld;
   const Grid<T> grid(z, a.V);
@@ -521,7 +538,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
   // the peers' shared memory may be written once all of them run
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const float w = a.weight ? a.weight[row] : 1.0f;
-  Record<J> r;
+  Record<J, 32> r;
   if (warp == 0) r.read(row, a);
   const int edge = rank == 0 && tid < 2 * N ? grid.edge(tid) : -1;  // the first CTA's
   const float xe = edge >= 0 ? to_f(z[edge]) : -INFINITY;
@@ -659,17 +676,29 @@ cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const Di
   return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a, per);
 }
 
+template <class T, int E, int G, int J, bool HARD>
+void distill_warp(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a, int rows,
+                  cudaStream_t s) {
+  constexpr int PER = WARPS * (32 / G);  // rows of a CTA
+  distill_warp_kernel<T, E, G, J, HARD>
+      <<<(rows + PER - 1) / PER, 32 * WARPS, 0, s>>>(z, ld, d, ldd, a, rows);
+}
+
 template <class T, int J, bool HARD>
 cudaError_t distill_launch(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                            int rows, cudaStream_t s) {
   const int V = a.V;  // at least the elements in pieces
-  const int grid = (rows + WARPS - 1) / WARPS, block = 32 * WARPS;
-  if (V <= 32 * 8)
-    distill_warp_kernel<T, 8, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+  if (J == 1 && V <= 32 * 8 && a.K <= 16 && rows >= 2048)
+    // two rows a warp (16384 rows of 256, top 16: 11.4 us, 13.1 with a row each; with
+    // labels 14.2 and 14.9; 1024 rows 4.8 and 4.5). A longer record would take two
+    // entries a lane, and the search for repeated indices more than it saves.
+    distill_warp<T, 16, 16, J, HARD>(z, ld, d, ldd, a, rows, s);
+  else if (V <= 32 * 8)
+    distill_warp<T, 8, 32, J, HARD>(z, ld, d, ldd, a, rows, s);
   else if (V <= 32 * 16)
-    distill_warp_kernel<T, 16, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+    distill_warp<T, 16, 32, J, HARD>(z, ld, d, ldd, a, rows, s);
   else if (V <= 32 * 32)
-    distill_warp_kernel<T, 32, J, HARD><<<grid, block, 0, s>>>(z, ld, d, ldd, a, rows);
+    distill_warp<T, 32, 32, J, HARD>(z, ld, d, ldd, a, rows, s);
   else if (V <= 256 * 8)
     distill_cta_kernel<T, 8, J, HARD><<<rows, 256, 0, s>>>(z, ld, d, ldd, a);
   else if (V <= 256 * 16)
