@@ -168,7 +168,10 @@ int rnet_scale_grads(float* grads, float scale, size_t n, void* stream);
  * Operators on the logits of a model (no counterpart in the reference). Rows
  * of logits are fp32 or bf16 with a pitch of `ld` elements (ld >= vocab, any
  * alignment of the element size). All arithmetic is fp32 or wider. A
- * temperature lies within 1e-4 and 1e4. */
+ * temperature lies within 1e-4 and 1e4. Nothing is kept from one call for the
+ * next, and calls on different streams share nothing but the device error word;
+ * that is set up by a device's first call, which is made outside any stream
+ * capture. */
 #define RNET_DTYPE_F32 0
 #define RNET_DTYPE_BF16 1
 
@@ -177,7 +180,7 @@ int rnet_scale_grads(float* grads, float scale, size_t n, void* stream);
  * top_k]; lse (may be NULL) is [rows]: log sum exp(logit / temperature) over
  * the whole row. A NaN logit counts as -inf, +inf as the largest finite fp32.
  * Places beyond the row's logits above -inf hold -inf / -1 (padding that the
- * distillation skips). */
+ * distillation skips). vocab is at most 2^30. */
 int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float temperature,
                              float* top_logits, int* top_idx, float* lse, int rows, int vocab,
                              int top_k, void* stream);
@@ -224,7 +227,8 @@ int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const
  * finite fp32; candidates at -inf are never taken. A sequence with fewer
  * candidates than beams fills the places left with score -inf, parent = the
  * place itself and token = eos (0 without one). So a search starts with scores
- * {0, -inf, ...}. scores / finished may be scores_in / finished_in. */
+ * {0, -inf, ...}. scores / finished may be scores_in / finished_in. vocab is at
+ * most 2^30. */
 int rnet_beam_select(const void* logits, int dtype, long long ld, const float* scores_in,
                      const int* finished_in, int eos, float* scores, int* tokens, int* parents,
                      int* finished, int batch, int beams, int vocab, void* stream);
@@ -245,8 +249,9 @@ int rnet_beam_reorder(const void* src, void* dst, size_t row_bytes, size_t row_p
  * beams sorted by score / length^length_alpha (64 bits, ties to the lower
  * beam); length counts the tokens up to and including the first eos (n_steps
  * without one, or with eos < 0), and eos fills what follows. lengths and
- * ranked_scores [batch * beams] are in the same order. A parent outside
- * 0..beams-1 counts as the beam itself and sets the device error word (bit 1). */
+ * ranked_scores [batch * beams] are in the same order (ranked_scores may be
+ * scores). A parent outside 0..beams-1 counts as the beam itself and sets the
+ * device error word (bit 1). */
 int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
                         float length_alpha, int* sequences, int* lengths, float* ranked_scores,
                         int n_steps, int batch, int beams, void* stream);

@@ -14,7 +14,8 @@ using namespace rnet_logits;
 // The best `beams` of score[b] + z[b][v] - lse[b] over (b, v): within a row the
 // order of the totals is that of the logits, so each row (or slice of a row)
 // gives its W largest logits and its sum of exponentials, and one warp merges
-// the sorted lists, a lane each. Totals are formed and compared in 64 bits.
+// the sorted lists, a lane each. Totals are formed and compared in 64 bits, score
+// and logit first: beams with the same row tie where their sums are equal.
 // What bounds it is HBM for long rows, latency for short ones.
 struct SelectArgs {
   const float* scores_in;
@@ -75,7 +76,7 @@ __device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size
     } else {
       const uint64_t k = in.key[lane][at];
       token = key_index(k);
-      total = score + ((double)key_value(k) - lse);
+      total = (score + (double)key_value(k)) - lse;  // the sum of two fp32 is exact, or near it
     }
     ++at;
   };

@@ -46,6 +46,7 @@ int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float 
   NEED(dtype == RNET_DTYPE_F32 || dtype == RNET_DTYPE_BF16,
        "topk_logits_forward: dtype must be RNET_DTYPE_F32 or RNET_DTYPE_BF16");
   NEED(rows >= 0 && vocab > 0, "topk_logits_forward: bad size");
+  NEED(vocab <= RNET_SELECT_VOCAB_MAX, "topk_logits_forward: vocab above 2^30");
   NEED(ld >= vocab, "topk_logits_forward: row pitch below vocab");
   NEED(top_k >= 1 && top_k <= RNET_TOPK_MAX && top_k <= vocab,
        "topk_logits_forward: " + TOPK_RANGE + " and not above vocab");
@@ -105,6 +106,7 @@ int rnet_beam_select(const void* logits, int dtype, long long ld, const float* s
   NEED(batch >= 0 && vocab > 0, "beam_select: bad size");
   NEED(beams >= 1 && beams <= RNET_BEAMS_MAX, "beam_select: " + BEAM_RANGE);
   NEED((long long)batch * beams <= 0x7fffffffLL, "beam_select: batch * beams too large");
+  NEED(vocab <= RNET_SELECT_VOCAB_MAX, "beam_select: vocab above 2^30");
   NEED(ld >= vocab, "beam_select: row pitch below vocab");
   NEED(eos >= -1 && eos < vocab, "beam_select: eos must be -1 (none) or a token");
   NEED(!finished_in || (eos >= 0 && finished),
@@ -154,6 +156,9 @@ int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scor
   NEED(aligned(tokens, 4) && aligned(parents, 4) && aligned(scores, 4) && aligned(sequences, 4) &&
            aligned(lengths, 4) && aligned(ranked_scores, 4),
        "beam_backtrack: a pointer is not aligned to its element size");
+  const size_t bytes = (size_t)n_steps * batch * beams * sizeof(int);
+  NEED(!overlap(sequences, bytes, tokens, bytes) && !overlap(sequences, bytes, parents, bytes),
+       "beam_backtrack: sequences overlap the records");
   CK(rnet_k::beam_backtrack(tokens, parents, scores, eos, length_alpha, sequences, lengths,
                             ranked_scores, n_steps, batch, beams, ew(), (cudaStream_t)stream));
   return RNET_OK;

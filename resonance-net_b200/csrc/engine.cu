@@ -842,6 +842,9 @@ int Engine::train_step_distill(const int* d_in, const int* t_idx, const float* t
     return rnet_status::fail(RNET_ERR_ARG,
                              "train_step_distill: batch*seq_len must be 1..64*seq_len");
   const int N = (int)tokens, V = cfg_.vocab_size;
+  if (V > RNET_DISTILL_VOCAB_MAX)
+    return rnet_status::fail(RNET_ERR_UNSUPPORTED, "train_step_distill: vocab above " +
+                                                       std::to_string(RNET_DISTILL_VOCAB_MAX));
   if (N > row_loss_cap_) {
     CK(cudaStreamSynchronize(stream_));
     cudaFree(row_loss_);

@@ -8,6 +8,7 @@
 #define RNET_TOPK_MAX 64
 #define RNET_BEAMS_MAX 32
 #define RNET_DISTILL_VOCAB_MAX 262144
+#define RNET_SELECT_VOCAB_MAX (1 << 30)
 
 namespace rnet_k {
 

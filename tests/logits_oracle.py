@@ -93,7 +93,8 @@ def distill(z, t_idx, t_val, tau, soft, hard, scale, t_lse=None, targets=None, w
         bl[r] = abs(w) * (bl[r] + abs(l) * 4 * U)
         bg[r] = abs(scale * w) * (bg[r] + np.abs(g) * 4 * U)
     # beyond the largest fp32 number a loss rounds to infinity
-    loss = np.where(np.abs(loss) > float(FMAX), np.sign(loss) * np.inf, loss)
+    over = np.abs(loss) > float(FMAX)
+    loss[over] = np.sign(loss[over]) * np.inf
     return loss, grad, bl, bg
 
 
@@ -105,7 +106,7 @@ def select(z, scores, beams, eos=-1, finished=None):
     b = m // beams
     s = canon(scores)
     with np.errstate(invalid="ignore"):
-        t = s[:, None] + (z - logsumexp(z)[:, None])
+        t = (s[:, None] + z) - logsumexp(z)[:, None]
     t = np.where((z == -np.inf) | (s[:, None] == -np.inf), -np.inf, t)
     done = np.zeros(m, bool) if finished is None else np.asarray(finished) != 0
     t[done] = -np.inf

@@ -49,7 +49,7 @@ def _check_select(rnet, torch, z, dtype, scores, beams, eos=-1, finished=None, g
     fin = np.isfinite(want[0])
     np.testing.assert_array_equal(got[0][~fin], want[0][~fin].astype(np.float32))
     bound = ref.lse_bound(want[0], z.shape[1]) + np.abs(np.where(fin, want[0], 0)) * ref.U
-    assert np.all(np.abs(got[0] - want[0])[fin] <= bound[fin])
+    assert np.all(np.abs(got[0][fin] - want[0][fin]) <= bound[fin])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -80,6 +80,35 @@ def test_select_ties_go_to_the_lowest_candidate(rnet, cuda, v):
     _check_select(rnet, torch, z, "f32", np.full(2 * beams, -1.5, np.float32), beams, eos=0)
     _check_select(rnet, torch, _logits(torch, np.zeros((beams, v), np.float32), "bf16"), "bf16",
                   np.zeros(beams, np.float32), beams)
+
+
+@pytest.mark.parametrize("v", [255, 1023, 2047, 30001])
+def test_select_ties_of_equal_bf16_rows(rnet, cuda, v):
+    """Rows that start on every 2-byte place of a 16-byte grid."""
+    torch, beams = cuda, 8
+    row = (np.random.default_rng(v).normal(size=(1, v)) * 2).astype(np.float32)
+    for offset in (0, 1):
+        z = _logits(torch, np.repeat(row, 2 * beams, 0), "bf16", 0, offset)
+        _check_select(rnet, torch, z, "bf16", np.full(2 * beams, -0.5, np.float32), beams)
+
+
+def test_many_sequences(rnet, cuda):
+    """More sequences than a grid's second dimension holds."""
+    torch, batch, beams, v = cuda, 70000, 2, 5
+    r = np.random.default_rng(0)
+    m = batch * beams
+    # equal rows and scores on a grid: two totals are equal or at least 1 / 64 apart,
+    # and equal ones come from different scores and logits
+    z = np.repeat(np.array([[2.0, 0.0, 4.0, 1.0, 3.0]], np.float32), m, 0)
+    scores = (-r.integers(0, 256, size=m) / 64.0).astype(np.float32)
+    _check_select(rnet, torch, _logits(torch, z, "f32"), "f32", scores, beams)
+    tok, par = r.integers(0, 9, size=(3, m)).astype(np.int32), r.integers(0, 2, size=(3, m)).astype(
+        np.int32)
+    seq, ln, rk = _backtrack(rnet, torch, tok, par, scores, beams, 3, 0.0)
+    s0, l0, r0 = ref.backtrack(tok, par, scores, beams, 3, 0.0)
+    np.testing.assert_array_equal(seq, s0)
+    np.testing.assert_array_equal(ln, l0)
+    np.testing.assert_array_equal(rk, r0.astype(np.float32))
 
 
 @pytest.mark.parametrize("v", [40, 700, 9000])
@@ -218,7 +247,7 @@ def test_backtrack(rnet, cuda, t, batch, beams, eos, alpha):
     np.testing.assert_array_equal(seq, s0)
     fin = np.isfinite(r0)
     np.testing.assert_array_equal(rk[~fin], r0[~fin])
-    assert np.all(np.abs(rk - r0)[fin] <= 2 * ref.U * np.abs(r0[fin]))
+    assert np.all(np.abs(rk[fin] - r0[fin]) <= 2 * ref.U * np.abs(r0[fin]))
 
 
 def test_backtrack_bad_parents(rnet, cuda):

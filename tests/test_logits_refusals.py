@@ -51,6 +51,7 @@ def _args(entry, base, change):
     ("rnet_topk_logits_forward", dict(rows=-1), "bad size"),
     ("rnet_topk_logits_forward", dict(vocab=0), "bad size"),
     ("rnet_topk_logits_forward", dict(ld=7), "row pitch"),
+    ("rnet_topk_logits_forward", dict(vocab=2 ** 30 + 1, ld=2 ** 31), "2^30"),
     ("rnet_topk_logits_forward", dict(k=0), "top_k"),
     ("rnet_topk_logits_forward", dict(k=9), "top_k"),
     ("rnet_topk_logits_forward", dict(vocab=100, ld=100, k=65), "top_k"),
@@ -81,6 +82,7 @@ def _args(entry, base, change):
     ("rnet_beam_select", dict(beams=0), "beams"),
     ("rnet_beam_select", dict(beams=33), "beams"),
     ("rnet_beam_select", dict(ld=7), "row pitch"),
+    ("rnet_beam_select", dict(vocab=2 ** 30 + 1, ld=2 ** 31), "2^30"),
     ("rnet_beam_select", dict(eos=8), "eos"),
     ("rnet_beam_select", dict(eos=-2), "eos"),
     ("rnet_beam_select", dict(f_in=1, fin=1), "eos"),
@@ -105,6 +107,8 @@ def _args(entry, base, change):
     ("rnet_beam_backtrack", dict(beams=40), "beams"),
     ("rnet_beam_backtrack", dict(alpha=float("nan")), "finite"),
     ("rnet_beam_backtrack", dict(seq=3), "aligned"),
+    ("rnet_beam_backtrack", dict(), "overlap"),
+    ("rnet_beam_backtrack", dict(seq=1025, tok=1029, par=2049), "overlap"),
 ])
 def test_refused(rnet, buf, entry, change, text):
     _refused(rnet, entry, _args(entry, buf[1], change), text)
