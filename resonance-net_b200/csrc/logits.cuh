@@ -66,13 +66,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-// log2 x, absolute error below 2^-22 near 1, relative 2^-22 elsewhere.
-__device__ __forceinline__ float log2_fast(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // The largest value of a warp; NaN loses against any number.
 __device__ __forceinline__ float warp_max(float v) {
   float y;

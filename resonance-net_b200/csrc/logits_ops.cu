@@ -138,7 +138,8 @@ struct RowGrad {
 template <int J, int G>
 struct Record {
   int idx[J];  // -1: no entry
-  float z[J], p[J], lp[J];  // student's logit, teacher's probability and its log
+  float z[J], p[J], lp[J];  // student's logit, teacher's probability, log2 p + ln / ln 2
+  float ln;    // log of the record's own normaliser
   int y;       // label, -1: none
   float zy;
   float P;     // sum p
@@ -175,49 +176,57 @@ struct Record {
     }
   }
   // Probabilities relative to the record's own maximum, or to the teacher's
-  // normaliser if it is given. An entry at -inf has none.
-  __device__ __forceinline__ void weigh(size_t row, const DistillArgs& a) {
+  // normaliser if it is given. An entry at -inf has none. They are taken to base 2
+  // with the same constant c as the student's terms, so that its rounding does not
+  // show in the difference of the two, which may be small (a student near its
+  // teacher); what is done once a row or entry here and in loss() is done with
+  // the accurate functions for the same reason.
+  __device__ __forceinline__ void weigh(size_t row, const DistillArgs& a, float c) {
     float tm = -INFINITY;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      lp[j] = idx[j] >= 0 ? lp[j] * a.inv_tau : -INFINITY;
+      if (idx[j] < 0) lp[j] = -INFINITY;
       tm = fmaxf(tm, lp[j]);
     }
     const bool given = a.t_lse != nullptr;
-    const float shift = given ? a.t_lse[row] : group_max<G>(tm);
+    const float lse = given ? a.t_lse[row] : 0.f;
+    if (!given) tm = group_max<G>(tm);
     float S = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const bool none = lp[j] == -INFINITY;
-      lp[j] -= shift;
-      p[j] = none ? 0.f : exp2_fast(lp[j] * LOG2E);
+      const float t = lp[j], d = t - tm;
+      lp[j] = given ? fmaf(t, c, -__fmul_rn(lse, LOG2E)) : d * c;
+      p[j] = t == -INFINITY ? 0.f : exp2f(lp[j]);
       S += p[j];
     }
     P = group_sum<G>(S);
+    ln = 0.f;
     if (given || P == 0.f) return;
-    const float inv = __fdividef(1.0f, P), ln = LN2 * log2_fast(P);
+    ln = logf(P);
+    const float inv = 1.0f / P;
 #pragma unroll
-    for (int j = 0; j < J; ++j) p[j] *= inv, lp[j] -= ln;
+    for (int j = 0; j < J; ++j) p[j] *= inv;
     P *= inv;
   }
-  // This lane's part of sum p (log p - term).
+  // This lane's part of sum p (lp - term).
   __device__ __forceinline__ float kl(float m, float c) const {
     float v = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (p[j] != 0.f) v += p[j] * (lp[j] - LN2 * term(z[j], m, c));
+      if (p[j] != 0.f) v += p[j] * (lp[j] - term(z[j], m, c));
     return v;
   }
-  // The row's loss from sum p (log p - term) and the sums of 2^term.
+  // The row's loss from sum p (lp - term) and the sums of 2^term.
   __device__ __forceinline__ float loss(const DistillArgs& a, float w, float kl, float m, float s,
                                         float s1) const {
     if (s == 0.f) return 0.f;  // every logit -inf: no distribution
     float l = 0.f;
     if (a.soft != 0.f) {
-      if (P != 0.f) kl += P * (LN2 * log2_fast(s));
+      kl *= LN2;
+      if (P != 0.f) kl += P * (logf(s) - ln);
       l = a.soft * a.tau * a.tau * kl;
     }
-    if (y >= 0) l += a.hard * (LN2 * (log2_fast(s1) - term(zy, m, LOG2E)));
+    if (y >= 0) l += a.hard * (logf(s1) - LN2 * term(zy, m, LOG2E));
     return w * l;
   }
   // The record's and the label's elements, those that are `in` this CTA's share,
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) dist
   const float c = a.inv_tau * LOG2E;
   Share<T, E, HARD> h;
   h.take(x, xe, c);
-  r.weigh(row, a);
+  r.weigh(row, a, c);
   const float m = group_max<G>(h.m);
   const float f = rebase(h.m, m, c), f1 = HARD ? rebase(h.m, m, LOG2E) : 0.f;
   const float s = group_sum<G>(h.s * f), s1 = HARD ? group_sum<G>(h.s1 * f1) : 0.f;
@@ -462,7 +471,7 @@ __global__ void __launch_bounds__(256) distill_cta_kernel(const T* logits, long 
   Share<T, E, HARD> h;
   h.take(x, xe, c);
   if (warp == 0) {
-    r.weigh(row, a);
+    r.weigh(row, a, c);
     if (lane == 0) s_P = r.P, s_label = r.y >= 0;
     if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   }
@@ -546,7 +555,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
   const float c = a.inv_tau * LOG2E;
   if (warp == 0) {
     r.gather(z, a.V);
-    r.weigh(row, a);
+    r.weigh(row, a, c);
     if (lane == 0) s_P = r.P, s_label = r.y >= 0;
     if (r.bad && rank == 0 && w != 0.f && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   }

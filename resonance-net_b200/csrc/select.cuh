@@ -103,7 +103,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 // log of the sum of exponentials at tau from the largest logit m and the sum s of
 // 2^((x - m) log2(e) / tau); -inf for a row without a logit above -inf.
 __device__ __forceinline__ float log_sum(float m, float s, float inv_tau) {
-  return s > 0.f ? m * inv_tau + LN2 * log2_fast(s) : -INFINITY;
+  return s > 0.f ? m * inv_tau + logf(s) : -INFINITY;
 }
 __device__ __forceinline__ double log_sum(float m, double s) {
   return s > 0.0 ? (double)m + log(s) : -(double)INFINITY;
