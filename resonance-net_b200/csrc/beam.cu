@@ -297,8 +297,9 @@ struct Segment {
   int W;
   bool on;         // this lane has a beam
 
-  // From beam a at step end - 1 to the first step; f(t, token) sees the tokens on
-  // the way. Returns the beam before the segment. `steps` is the same in all lanes.
+  // From beam a at step end - 1 to the first step; f(t, tokens) sees the tokens of
+  // steps t - 1, .. t - BACK on the way (those below `begin` are not the segment's).
+  // Returns the beam before the segment. `steps` is the same in all lanes.
   template <bool TOKENS, class F>
   __device__ __forceinline__ int walk(int steps, int a, bool& bad, F f) const {
     const int own = (threadIdx.x & 31) - first;
@@ -314,12 +315,10 @@ struct Segment {
 #pragma unroll
       for (int i = 0; i < BACK; ++i) {
         if (on && (p[i] < 0 || p[i] >= W)) p[i] = own, bad = true;
-        if (TOKENS) {
-          const int t = end - 1 - k - i, token = __shfl_sync(~0u, v[i], first + a);
-          if (t >= begin) f(t, token);
-        }
+        if (TOKENS) v[i] = __shfl_sync(~0u, v[i], first + a);
         a = __shfl_sync(~0u, p[i], first + a);
       }
+      if (TOKENS) f(end - k, v);
     }
     return a;
   }
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
   sg.parents = parents + m0 + beam;
   sg.tokens = tokens + m0 + beam;
   bool bad = false;
-  const int before = sg.walk<false>(steps, beam, bad, [](int, int) {});
+  const int before = sg.walk<false>(steps, beam, bad, [](int, int*) {});
   if (bad && err) atomicOr(err, rnet_dev::ERR_BAD_INDEX);
   // this segment's start for every beam at the end of the warp's last segment
   int a = beam, start = beam;
@@ -367,8 +366,10 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
   start = __shfl_sync(~0u, start, sg.first + from[warp][beam]);
   int len = T;
   if (eos >= 0) {
-    sg.walk<true>(steps, start, bad, [&](int t, int token) {
-      if (token == eos) len = t + 1;
+    sg.walk<true>(steps, start, bad, [&](int t, const int* token) {
+#pragma unroll
+      for (int i = 0; i < BACK; ++i)
+        if (t - 1 - i >= sg.begin && token[i] == eos) len = t - i;
     });
     for (int o = P; o < 32; o <<= 1) len = min(len, __shfl_xor_sync(~0u, len, o));
     ends[warp][lane] = len;
@@ -394,8 +395,23 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
   __syncthreads();
   len = s_len[beam];
   int* out = seq + (m0 + (sg.on ? s_rank[beam] : 0)) * T;
-  sg.walk<true>(steps, start, bad, [&](int t, int token) {
-    if (sg.on) out[t] = t >= len ? eos : token;
+  sg.walk<true>(steps, start, bad, [&](int t, int* token) {
+    if (!sg.on) return;
+#pragma unroll
+    for (int i = 0; i < BACK; ++i)
+      if (t - 1 - i >= len) token[i] = eos;
+    int* to = out + t - BACK;
+    if (t - BACK >= sg.begin && ((uintptr_t)to & 15) == 0) {
+      // 32 bytes of one sequence at a time: a sector is written once
+#pragma unroll
+      for (int i = BACK - 4; i >= 0; i -= 4)
+        *reinterpret_cast<int4*>(to + BACK - 4 - i) =
+            make_int4(token[i + 3], token[i + 2], token[i + 1], token[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < BACK; ++i)
+        if (t - 1 - i >= sg.begin) out[t - 1 - i] = token[i];
+    }
   });
 }
 
@@ -491,7 +507,8 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
   const int per_warp = 32 / P;
   int warps = (steps + BACK * per_warp - 1) / (BACK * per_warp);
   if (warps > BACK_WARPS) warps = BACK_WARPS;
-  const int per = (steps + warps * per_warp - 1) / (warps * per_warp);
+  int per = (steps + warps * per_warp - 1) / (warps * per_warp);
+  per = (per + BACK - 1) / BACK * BACK;  // whole batches, which start on a multiple of BACK
   beam_backtrack_kernel<<<batch, 32 * warps, 0, s>>>(tokens, parents, scores, eos, alpha,
                                                      sequences, lengths, ranked, steps,
                                                      (size_t)batch * beams, beams, P, per, err);
