@@ -287,6 +287,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(
 // the right beams, first for the first eos, then to write. What bounds it is the
 // latency of one segment's loads and shuffles, three times.
 constexpr int BACK_WARPS = 32;
+constexpr int BACK_CTAS = 8;
 constexpr int BACK = 8;  // steps whose loads are under way together
 
 struct Segment {
@@ -324,26 +325,41 @@ struct Segment {
   }
 };
 
+__device__ __forceinline__ void store_int_in(int* p, int rank, int v) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "st.shared::cluster.u32 [ra], %2;\n\t}" ::"r"(rnet_dev::smem_u32(p)),
+      "r"(rank), "r"(v)
+      : "memory");
+}
+
+// A cluster of CTAs per sequence (one where they have enough segments).
 __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
-    const int* __restrict__ tokens, const int* __restrict__ parents,
-    const float* __restrict__ scores, int eos, float alpha, int* __restrict__ seq,
-    int* __restrict__ lengths, float* __restrict__ ranked, int T, size_t M, int W, int P,
-    int steps, unsigned* err) {
+    const int* __restrict__ tokens, const int* __restrict__ parents, const float* scores, int eos,
+    float alpha, int* __restrict__ seq, int* __restrict__ lengths, float* ranked, int T, size_t M,
+    int W, int P, int steps, unsigned* err) {
   rnet_dev::pdl_trigger();
   __shared__ int map[BACK_WARPS][32], from[BACK_WARPS][32], ends[BACK_WARPS][32];
-  __shared__ int s_len[32], s_rank[32];
+  __shared__ int cta_map[BACK_CTAS][32], cta_len[BACK_CTAS][32];
+  __shared__ int s_start[32], s_len[32], s_rank[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int cta = blockIdx.y, ctas = gridDim.y;
   const int G = 32 / P, beam = lane & (P - 1), part = lane / P;
   const size_t m0 = (size_t)blockIdx.x * W;
+  // the peers' shared memory may be written once all of them run
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   Segment sg;
   sg.M = M;
   sg.W = W;
   sg.first = lane - beam;
   sg.on = beam < W;
-  sg.begin = min((warp * G + part) * steps, T);
+  sg.begin = (int)min((long long)((cta * warps + warp) * G + part) * steps, (long long)T);
   sg.end = min(sg.begin + steps, T);
   sg.parents = parents + m0 + beam;
   sg.tokens = tokens + m0 + beam;
+  // read before the first exchange: the ranked scores may take its place
+  const float score = sg.on ? scores[m0 + beam] : 0.f;
   bool bad = false;
   const int before = sg.walk<false>(steps, beam, bad, [](int, int*) {});
   if (bad && err) atomicOr(err, rnet_dev::ERR_BAD_INDEX);
@@ -355,15 +371,24 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
   }
   map[warp][lane] = a;  // the same in all parts
   __syncthreads();
-  if (warp == 0) {
+  if (ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (warp == 0) {  // the same over the CTA's warps, for every beam at its end
     int b = beam;
     for (int k = warps - 1; k >= 0; --k) {
       from[k][lane] = b;
       b = map[k][b];
     }
+    if (ctas > 1)
+      for (int r = 0; r < ctas; ++r) store_int_in(&cta_map[cta][lane], r, b);
+  }
+  if (ctas > 1) rnet_dev::cluster_sync();
+  if (warp == 0) {  // and over the CTAs behind this one
+    int b = beam;
+    for (int r = ctas - 1; r > cta; --r) b = cta_map[r][b];
+    s_start[lane] = b;
   }
   __syncthreads();
-  start = __shfl_sync(~0u, start, sg.first + from[warp][beam]);
+  start = __shfl_sync(~0u, start, sg.first + from[warp][s_start[beam]]);
   int len = T;
   if (eos >= 0) {
     sg.walk<true>(steps, start, bad, [&](int t, const int* token) {
@@ -374,12 +399,19 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
     for (int o = P; o < 32; o <<= 1) len = min(len, __shfl_xor_sync(~0u, len, o));
     ends[warp][lane] = len;
     __syncthreads();
+    if (warp == 0) {
+      for (int k = 0; k < warps; ++k) len = min(len, ends[k][lane]);
+      if (ctas > 1)
+        for (int r = 0; r < ctas; ++r) store_int_in(&cta_len[cta][lane], r, len);
+    }
+    if (ctas > 1) {
+      rnet_dev::cluster_sync();
+      for (int r = 0; r < ctas; ++r) len = min(len, cta_len[r][lane]);
+    }
   }
   if (warp == 0) {
-    if (eos >= 0)
-      for (int k = 0; k < warps; ++k) len = min(len, ends[k][lane]);
-    const double r = sg.on ? (double)canon(scores[m0 + beam]) / pow((double)len, (double)alpha)
-                           : -(double)INFINITY;
+    const double r =
+        sg.on ? (double)canon(score) / pow((double)len, (double)alpha) : -(double)INFINITY;
     int rank = 0;
     for (int i = 0; i < W; ++i) {
       const double o = __shfl_sync(~0u, r, i);
@@ -387,7 +419,7 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
     }
     s_len[lane] = len;
     s_rank[lane] = rank;
-    if (lane < W) {
+    if (lane < W && cta == 0) {
       lengths[m0 + rank] = len;
       ranked[m0 + rank] = (float)r;
     }
@@ -503,16 +535,21 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
   if (batch <= 0) return cudaSuccess;
   int P = 1;
   while (P < beams) P *= 2;
-  // segments of at least BACK steps
+  // segments of at least BACK steps; eight warps of them to a CTA while a cluster of
+  // CTAs finds idle SMs (4 sequences of 4096 steps: 7.3 us, 19.4 in one CTA each)
   const int per_warp = 32 / P;
   int warps = (steps + BACK * per_warp - 1) / (BACK * per_warp);
+  int ctas = 1;
+  while (ctas < BACK_CTAS && warps > 8 * ctas && (long long)batch * 2 * ctas <= 148) ctas *= 2;
+  warps = (warps + ctas - 1) / ctas;
   if (warps > BACK_WARPS) warps = BACK_WARPS;
-  int per = (steps + warps * per_warp - 1) / (warps * per_warp);
+  const int segments = ctas * warps * per_warp;
+  int per = (steps + segments - 1) / segments;
   per = (per + BACK - 1) / BACK * BACK;  // whole batches, which start on a multiple of BACK
-  beam_backtrack_kernel<<<batch, 32 * warps, 0, s>>>(tokens, parents, scores, eos, alpha,
-                                                     sequences, lengths, ranked, steps,
-                                                     (size_t)batch * beams, beams, P, per, err);
-  return launched();
+  const cudaError_t e = launch_cluster(beam_backtrack_kernel, batch, ctas, 32 * warps, 0, s, tokens,
+                                       parents, scores, eos, alpha, sequences, lengths, ranked,
+                                       steps, (size_t)batch * beams, beams, P, per, err);
+  return e != cudaSuccess ? e : launched();
 }
 
 }  // namespace rnet_k

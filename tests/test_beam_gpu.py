@@ -250,6 +250,24 @@ def test_backtrack(rnet, cuda, t, batch, beams, eos, alpha):
     assert np.all(np.abs(rk[fin] - r0[fin]) <= 2 * ref.U * np.abs(r0[fin]))
 
 
+def test_backtrack_ranks_in_place(rnet, cuda):
+    """The ranked scores may take the scores' place."""
+    torch, t, m, beams = cuda, 3000, 6, 3
+    r = np.random.default_rng(4)
+    tok = r.integers(0, 4000, size=(t, m)).astype(np.int32)
+    par = r.integers(0, beams, size=(t, m)).astype(np.int32)
+    scores = (-10 * r.random(m)).astype(np.float32)
+    want = _backtrack(rnet, torch, tok, par, scores, beams, 5, 0.4)
+    T, P, S = _t(torch, tok), _t(torch, par), _t(torch, scores)
+    seq = torch.empty(m, t, dtype=torch.int32, device="cuda")
+    ln = torch.empty(m, dtype=torch.int32, device="cuda")
+    rnet.call("rnet_beam_backtrack", T.data_ptr(), P.data_ptr(), S.data_ptr(), 5, 0.4,
+              seq.data_ptr(), ln.data_ptr(), S.data_ptr(), t, m // beams, beams, None)
+    torch.cuda.synchronize()
+    for x, y in zip((seq, ln, S), want):
+        np.testing.assert_array_equal(x.cpu().numpy(), y)
+
+
 def test_backtrack_bad_parents(rnet, cuda):
     rnet.device_error(clear=True)
     tok = np.arange(12, dtype=np.int32).reshape(4, 3)
