@@ -520,26 +520,29 @@ __device__ __forceinline__ void store_remote(float4* p, uint32_t rank, float4 v)
       : "memory");
 }
 
-constexpr int CLUSTER = 8;      // CTAs of one row at most
-constexpr int LONG = 512;       // their threads
-constexpr int CHUNK = 4 * LONG; // pieces (32 KB) that arrive together
+constexpr int CLUSTER = 8;  // CTAs of one row at most
 constexpr int CHUNKS = 5;
-// Pieces of a row in one CTA's shared memory, so that two CTAs share an SM and
-// one reads while the other computes and writes.
-constexpr int SHARE = 108 * 1024 / 16;
-static_assert(RNET_DISTILL_VOCAB_MAX * 4 / 16 <= CLUSTER * CHUNK * CHUNKS, "vocab limit");
+// Pieces of a row in one CTA's shared memory, so that two CTAs of 512 threads share
+// an SM and one reads while the other computes and writes; with 256 threads, four
+// (4096 rows of 10000 fp32: 56.4 us, 79.1 with 512 threads).
+constexpr int SHARE = 108 * 1024 / 16, SHARE_256 = 54 * 1024 / 16;
+// Pieces that arrive together, 64 bytes a thread.
+template <int NT>
+constexpr int CHUNK = 4 * NT;
+static_assert(RNET_DISTILL_VOCAB_MAX * 4 / 16 <= CLUSTER * CHUNK<512> * CHUNKS, "vocab limit");
+static_assert(SHARE_256 <= CHUNK<256> * CHUNKS, "share limit");
 
 // Longer rows: a cluster of C CTAs per row, each with `per` pieces in shared
 // memory. Chunks of the row arrive by bulk copies, and their maxima and sums are
 // taken as they do. Every warp leaves its own in the shared memory of all CTAs of
 // the cluster: one exchange, and the same bits everywhere. The gradient is then
 // computed from shared memory. Warp 0 of each CTA holds the record.
-template <class T, int J, bool HARD>
-__global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, long long ld,
-                                                               T* dlogits, long long ldd,
-                                                               DistillArgs a, int per) {
+template <class T, int NT, int J, bool HARD>
+__global__ void __launch_bounds__(NT, 1024 / NT)
+    distill_long_kernel(const T* logits, long long ld, T* dlogits, long long ldd, DistillArgs a,
+                        int per) {
   rnet_dev::pdl_trigger();
-  constexpr int N = Piece<T>::N, NW = LONG / 32;
+  constexpr int N = Piece<T>::N, NW = NT / 32, CH = CHUNK<NT>;
   extern __shared__ uint4 long_buf[];
   Piece<T>* const buf = reinterpret_cast<Piece<T>*>(long_buf);
   __shared__ float4 part[CLUSTER * NW];  // m, s, s1
@@ -556,10 +559,10 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
     s_abort[0] = s_abort[1] = 0;
     for (int i = 0; i < CHUNKS; ++i) rnet_dev::mbar_init(&bar[i], 1);
     rnet_dev::fence_barrier_init();
-    for (int i = 0; i * CHUNK < n; ++i) {
-      const uint32_t bytes = 16u * min(CHUNK, n - i * CHUNK);
+    for (int i = 0; i * CH < n; ++i) {
+      const uint32_t bytes = 16u * min(CH, n - i * CH);
       rnet_dev::mbar_arrive_expect_tx(&bar[i], bytes);
-      bulk_load(buf + i * CHUNK, z + grid.at(begin + i * CHUNK), bytes, &bar[i]);
+      bulk_load(buf + i * CH, z + grid.at(begin + i * CH), bytes, &bar[i]);
     }
   }
   // the peers' shared memory may be written once all of them run
@@ -597,7 +600,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
     }
   };
   if (edge >= 0) add(fmaxf(m, xe), [&](auto f) { f(xe); });
-  for (int i = 0; i * CHUNK < n; ++i) {
+  for (int i = 0; i * CH < n; ++i) {
     // a copy that does not come is reported and given the same time once more:
     // none may land in memory that the CTA has left
     if (!rnet_dev::mbar_wait(&bar[i], 0, a.err, &s_abort[0]))
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
     Piece<T> x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int q = i * CHUNK + j * LONG + tid;
+      const int q = i * CH + j * NT + tid;
       x[j].none();
       if (q < n) x[j] = buf[q];
     }
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
     __syncthreads();
   }
   if (w == 0.f) {  // whatever the row holds
-    if (d) zero_pieces(d, grid, begin + tid, LONG, begin + n, edge);
+    if (d) zero_pieces(d, grid, begin + tid, NT, begin + n, edge);
     if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
     return;
   }
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
   T* p = d + grid.at(begin);
   auto write = [&](bool wide, auto value) {
 #pragma unroll 2
-    for (int q = tid; q < n; q += LONG) {
+    for (int q = tid; q < n; q += NT) {
       const Piece<T> x = buf[q];
       float v[N];
 #pragma unroll
@@ -675,23 +678,18 @@ __global__ void __launch_bounds__(LONG, 2) distill_long_kernel(const T* logits, 
   }
 }
 
-template <class T, int J, bool HARD>
-cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
-                         int rows, cudaStream_t s) {
-  auto kernel = distill_long_kernel<T, J, HARD>;
-  const int pieces = a.V / Piece<T>::N;
-  int C = (pieces + SHARE - 1) / SHARE;
-  // more CTAs while they would leave SMs idle and have two chunks each
-  while (C < CLUSTER && (long long)rows * (C + 1) <= 148 && pieces / (C + 1) >= 2 * LONG) ++C;
-  if (C > CLUSTER) C = CLUSTER;
-  const int per = (pieces + C - 1) / C;
-  if (per > CHUNK * CHUNKS) return cudaErrorInvalidValue;
+template <class T, int NT, int J, bool HARD>
+cudaError_t distill_long_as(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
+                            int rows, int C, cudaStream_t s) {
+  auto kernel = distill_long_kernel<T, NT, J, HARD>;
+  const int per = (a.V / Piece<T>::N + C - 1) / C;
+  if (per > CHUNK<NT> * CHUNKS) return cudaErrorInvalidValue;
   static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem((const void*)kernel, 16 * CHUNK * CHUNKS, ready);
+  cudaError_t e = allow_smem((const void*)kernel, 16 * CHUNK<NT> * CHUNKS, ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows, C);
-  cfg.blockDim = dim3(LONG);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = (size_t)per * 16;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -701,6 +699,19 @@ cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const Di
   cfg.attrs = at;
   cfg.numAttrs = C > 1;
   return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a, per);
+}
+
+template <class T, int J, bool HARD>
+cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
+                         int rows, cudaStream_t s) {
+  const int pieces = a.V / Piece<T>::N;
+  int C = (pieces + SHARE - 1) / SHARE;
+  // more CTAs while they would leave SMs idle and have two chunks each
+  while (C < CLUSTER && (long long)rows * (C + 1) <= 148 && pieces / (C + 1) >= 1024) ++C;
+  if (C > CLUSTER) C = CLUSTER;
+  return (pieces + C - 1) / C <= SHARE_256 && rows > 148
+             ? distill_long_as<T, 256, J, HARD>(z, ld, d, ldd, a, rows, C, s)
+             : distill_long_as<T, 512, J, HARD>(z, ld, d, ldd, a, rows, C, s);
 }
 
 template <class T, int E, int G, int J, bool HARD>
