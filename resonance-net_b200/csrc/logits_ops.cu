@@ -705,7 +705,10 @@ template <class T, int J, bool HARD>
 cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                          int rows, cudaStream_t s) {
   const int pieces = a.V / Piece<T>::N;
-  int C = (pieces + SHARE - 1) / SHARE;
+  // one CTA while the row fits one, else shares of the smaller size (2048 rows of
+  // 30000 fp32: 90.5 us in three CTAs, 106 in two)
+  int C = pieces <= SHARE ? 1 : (pieces + SHARE_256 - 1) / SHARE_256;
+  if (C > CLUSTER) C = (pieces + SHARE - 1) / SHARE;
   // more CTAs while they would leave SMs idle and have two chunks each
   while (C < CLUSTER && (long long)rows * (C + 1) <= 148 && pieces / (C + 1) >= 1024) ++C;
   if (C > CLUSTER) C = CLUSTER;
