@@ -244,7 +244,7 @@ int rnet_beam_reorder(const void* src, void* dst, size_t row_bytes, size_t row_p
                       size_t outer_pitch, const int* parents, int batch, int beams, void* stream);
 
 /* The sequences behind the last beams. tokens / parents [n_steps, batch *
- * beams] are the recorded outputs of n_steps >= 1 selections, scores [batch *
+ * beams] are the recorded outputs of n_steps (1..2^30) selections, scores [batch *
  * beams] the last one's. sequences [batch * beams, n_steps]: per sequence the
  * beams sorted by score / length^length_alpha (64 bits, ties to the lower
  * beam); length counts the tokens up to and including the first eos (n_steps

@@ -72,6 +72,8 @@ int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const
   NEED(rows >= 0 && vocab > 0, "distill_topk_forward: bad size");
   NEED(ld >= vocab && (!dlogits || ld_dlogits >= vocab),
        "distill_topk_forward: row pitch below vocab");
+  NEED(rows == 0 || (ld <= (1LL << 60) / rows && (!dlogits || ld_dlogits <= (1LL << 60) / rows)),
+       "distill_topk_forward: row pitch too large");
   if (vocab > RNET_DISTILL_VOCAB_MAX)
     return rnet_status::fail(RNET_ERR_UNSUPPORTED,
                              "distill_topk_forward: vocab above " +
@@ -149,7 +151,7 @@ int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scor
                         int n_steps, int batch, int beams, void* stream) {
   NEED(tokens && parents && scores && sequences && lengths && ranked_scores,
        "beam_backtrack: null pointer");
-  NEED(n_steps >= 1 && batch >= 0, "beam_backtrack: bad size");
+  NEED(n_steps >= 1 && n_steps <= (1 << 30) && batch >= 0, "beam_backtrack: bad size");
   NEED(beams >= 1 && beams <= RNET_BEAMS_MAX, "beam_backtrack: " + BEAM_RANGE);
   NEED((long long)batch * beams <= 0x7fffffffLL, "beam_backtrack: batch * beams too large");
   NEED(std::isfinite(length_alpha), "beam_backtrack: length_alpha must be finite");

@@ -208,25 +208,34 @@ struct Record {
     for (int j = 0; j < J; ++j) p[j] *= inv;
     P *= inv;
   }
-  // This lane's part of sum p (lp - term).
-  __device__ __forceinline__ float kl(float m, float c) const {
+  // tau ln(2) term(x, m, c), in the logits' own unit: where the term itself leaves
+  // fp32 (a logit masked with the type's lowest value) it is the difference.
+  static __device__ __forceinline__ float unit(float x, float m, float c, float tau) {
+    const float t = term(x, m, c);
+    return t == -INFINITY && x > -INFINITY ? x - m : tau * (LN2 * t);
+  }
+  // This lane's part of tau sum p (ln(2) lp - ln(2) term).
+  __device__ __forceinline__ float kl(float m, float c, float tau) const {
     float v = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (p[j] != 0.f) v += p[j] * (lp[j] - term(z[j], m, c));
+      if (p[j] != 0.f) {
+        const float t = term(z[j], m, c);
+        v += p[j] * (t > -INFINITY ? tau * (LN2 * (lp[j] - t))
+                                   : tau * (LN2 * lp[j]) - unit(z[j], m, c, tau));
+      }
     return v;
   }
-  // The row's loss from sum p (lp - term) and the sums of 2^term.
+  // The row's loss from that sum and the sums of 2^term.
   __device__ __forceinline__ float loss(const DistillArgs& a, float w, float kl, float m, float s,
                                         float s1) const {
     if (s == 0.f) return 0.f;  // every logit -inf: no distribution
     float l = 0.f;
     if (a.soft != 0.f) {
-      kl *= LN2;
-      if (P != 0.f) kl += P * (logf(s) - ln);
-      l = a.soft * a.tau * a.tau * kl;
+      if (P != 0.f) kl += a.tau * (P * (logf(s) - ln));
+      l = a.soft * a.tau * kl;
     }
-    if (y >= 0) l += a.hard * (logf(s1) - LN2 * term(zy, m, LOG2E));
+    if (y >= 0) l += a.hard * (logf(s1) - unit(zy, m, LOG2E, 1.0f));
     return w * l;
   }
   // The record's and the label's elements, those that are `in` this CTA's share,
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) dist
   const float m = group_max<G>(h.m);
   const float f = rebase(h.m, m, c), f1 = HARD ? rebase(h.m, m, LOG2E) : 0.f;
   const float s = group_sum<G>(h.s * f), s1 = HARD ? group_sum<G>(h.s1 * f1) : 0.f;
-  const float kl = group_sum<G>(r.kl(m, c));
+  const float kl = group_sum<G>(r.kl(m, c, a.tau));
   if (lane == 0 && on) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   if (!dlogits) return;
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(256) distill_cta_kernel(const T* logits, long 
   __syncthreads();
   join_parts<1, HARD>(part, 8, c, m, s, s1);
   if (warp == 0) {
-    const float kl = warp_sum(r.kl(m, c));
+    const float kl = warp_sum(r.kl(m, c, a.tau));
     if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;
@@ -641,7 +650,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   }
   join_parts<CLUSTER * NW / 32, HARD>(part, C * NW, c, m, s, s1);
   if (rank == 0 && warp == 0) {
-    const float kl = warp_sum(r.kl(m, c));
+    const float kl = warp_sum(r.kl(m, c, a.tau));
     if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;

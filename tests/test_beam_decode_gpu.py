@@ -135,6 +135,25 @@ def test_one_beam_is_greedy_and_searches_repeat(rnet, rdata, cuda):
     m.close()
 
 
+def test_a_search_of_one_step(rnet, rdata, cuda):
+    """The best tokens of each prompt, by the logits of the prefill."""
+    torch = cuda
+    cfg, p, prompts = params_and_prompts(rnet, rdata)
+    m, dec = _decoder(rnet, torch, cfg, p, prompts, BEAMS)
+    lg, _ = dec.outputs_host()
+    seq, ln, sc = _search(torch, m, dec, BEAMS, 1)
+    for g in range(BATCH):
+        x = lg[g * BEAMS].astype(np.float64)
+        best = np.argsort(-x, kind="stable")[:BEAMS]
+        rows = slice(g * BEAMS, (g + 1) * BEAMS)
+        np.testing.assert_array_equal(seq[rows, 0], best)
+        lp = x[best] - ref.logsumexp(x)
+        assert np.all(np.abs(sc[rows] - lp) <= ref.lse_bound(lp, V) + np.abs(lp) * ref.U)
+    assert np.all(ln == 1)
+    dec.close()
+    m.close()
+
+
 def test_the_streams_hold_the_beams_afterwards(rnet, rdata, orc, cuda):
     """step(None) after a search feeds the last tokens: the logits are those of the
     whole sequences (with length_alpha 0 the ranking is the streams' order)."""

@@ -278,6 +278,32 @@ def test_distill_masked_rows_and_logits(rnet, cuda, v):
     assert got[0][5] == 0.0 and np.all(got[2][5] == 0.0)  # its neighbours are as before
 
 
+@pytest.mark.parametrize("v", [100, 900, 5000, 40000])
+@pytest.mark.parametrize("tau", [0.01, 1.0, 100.0])
+def test_distill_huge_logits_and_extreme_temperatures(rnet, cuda, v, tau):
+    """Logits up to the largest numbers, whose products with 1 / temperature leave
+    fp32: only their differences count."""
+    torch, n, k = cuda, 6, 5
+    r = np.random.default_rng(v)
+    z = (r.normal(size=(n, v)) * 2).astype(np.float32)
+    big = np.float32(3.0e38)
+    z[0, 3], z[0, 7] = big, big
+    z[1] = -big
+    z[2, ::2] = -big
+    z[3, 1:] = -np.inf
+    z[3, 0] = big
+    z[4] = np.float32(1e35)
+    idx = np.tile(np.array([3, 7, 0, 9, 11], np.int32), (n, 1))
+    idx[3] = [0, -1, -1, -1, -1]
+    idx[0, 2:] = -1
+    val = r.normal(size=(n, k)).astype(np.float32)
+    targets = np.array([7, 1, 1, 0, 2, 3], np.int32)
+    _, zz = _place(torch, z, "f32")
+    want = ref.distill(z, idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
+    got = _distill(rnet, torch, zz, "f32", idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
+    _check("f32", got, want)
+
+
 def test_distill_reports_indices_beyond_the_vocabulary(rnet, cuda):
     torch, n, v, k = cuda, 5, 300, 4
     r = np.random.default_rng(1)

@@ -68,6 +68,8 @@ def _args(entry, base, change):
     ("rnet_distill_topk_forward", dict(rows=-3), "bad size"),
     ("rnet_distill_topk_forward", dict(ld=1), "row pitch"),
     ("rnet_distill_topk_forward", dict(dlogits=2049, ldd=7), "row pitch"),
+    ("rnet_distill_topk_forward", dict(ld=2 ** 61), "too large"),
+    ("rnet_distill_topk_forward", dict(dlogits=2049, ldd=2 ** 61), "too large"),
     ("rnet_distill_topk_forward", dict(k=65), "top_k"),
     ("rnet_distill_topk_forward", dict(tau=-1.0), "temperature"),
     ("rnet_distill_topk_forward", dict(soft=float("inf")), "finite"),
@@ -104,6 +106,7 @@ def _args(entry, base, change):
       for p in ("tok", "par", "s", "seq", "ln", "rk")],
     ("rnet_beam_backtrack", dict(steps=0), "bad size"),
     ("rnet_beam_backtrack", dict(batch=-1), "bad size"),
+    ("rnet_beam_backtrack", dict(steps=2 ** 30 + 1), "bad size"),
     ("rnet_beam_backtrack", dict(beams=40), "beams"),
     ("rnet_beam_backtrack", dict(alpha=float("nan")), "finite"),
     ("rnet_beam_backtrack", dict(seq=3), "aligned"),
