@@ -13,9 +13,9 @@ using namespace rnet_logits;
 // ---------------------------------------------------------------- selection
 // The best `beams` of score[b] + z[b][v] - lse[b] over (b, v): within a row the
 // order of the totals is that of the logits, so each row (or slice of a row)
-// gives its W largest logits and its sum of exponentials, and one warp merges
-// the sorted lists, a lane each. Totals are formed and compared in 64 bits, score
-// and logit first: beams with the same row tie where their sums are equal.
+// gives its W largest logits and its sum of exponentials, and one CTA merges the
+// lists. Totals are formed and compared in 64 bits, score and logit first: beams
+// with the same row tie where their sums are equal.
 // What bounds it is HBM for long rows, latency for short ones.
 struct SelectArgs {
   const float* scores_in;
@@ -27,13 +27,18 @@ struct SelectArgs {
   unsigned* err;
 };
 
-// A list per (beam, slice), in that order, so that of equal totals the lowest
-// lane's is the lowest candidate.
+// A list per (beam, slice), in that order, largest first.
 struct Lists {
   uint64_t key[RNET_BEAMS_MAX][RNET_BEAMS_MAX];
   double s[RNET_BEAMS_MAX];
   float m[RNET_BEAMS_MAX];
   int n[RNET_BEAMS_MAX];
+  // the merge's own
+  uint64_t total[RNET_BEAMS_MAX * RNET_BEAMS_MAX];
+  int which[RNET_BEAMS_MAX * RNET_BEAMS_MAX];  // 32 list + place: the order of equal totals
+  double score[RNET_BEAMS_MAX], lse[RNET_BEAMS_MAX];
+  uint32_t done, bound;
+  int totals;
 };
 
 __device__ __forceinline__ uint64_t order(double x) {
@@ -41,63 +46,112 @@ __device__ __forceinline__ uint64_t order(double x) {
   return (uint64_t)b ^ ((uint64_t)(b >> 63) | 0x8000000000000000ull);
 }
 
-// One warp: W rounds over the heads of the W * S lists.
-__device__ __forceinline__ void merge(const Lists& in, const SelectArgs& a, size_t m0, int S) {
-  const int lane = threadIdx.x & 31, W = a.W;
-  const int beam = lane / S, part = lane % S;
-  const bool on = lane < W * S;
-  double score = -INFINITY, lse = 0.0;
+__device__ __forceinline__ double unorder(uint64_t o) {
+  return __longlong_as_double((int64_t)(o >> 63 ? o ^ 0x8000000000000000ull : ~o));
+}
+
+// What lane l of the first warp knows of list l's beam. Loaded ahead of the lists, so
+// that the merge does not wait for it.
+struct Standing {
+  float score = 0.f;
   bool done = false;
-  int n = 0;
-  if (on) {
-    score = canon(a.scores_in[m0 + beam]);
-    done = a.finished_in && a.finished_in[m0 + beam];
-    if (done) {
-      n = part == 0;  // (beam, eos) at its own score
-    } else {
-      n = in.n[lane];
-      float m = in.m[beam * S];
-      for (int i = 1; i < S; ++i) m = fmaxf(m, in.m[beam * S + i]);
-      double s = 0.0;
-      for (int i = 0; i < S; ++i)
-        s += in.s[beam * S + i] * (double)exp2_fast((in.m[beam * S + i] - m) * LOG2E);
-      lse = log_sum(m, s);
-    }
+  __device__ __forceinline__ void load(const SelectArgs& a, size_t m0, int S) {
+    const int lane = threadIdx.x & 31;
+    if (lane >= a.W * S) return;
+    score = a.scores_in[m0 + lane / S];
+    done = a.finished_in && a.finished_in[m0 + lane / S];
   }
-  __syncwarp();  // every input is read before the outputs, which may be the inputs
-  int at = 0, token = 0;
-  double total = -INFINITY;
-  auto next = [&]() {
-    total = -INFINITY;
-    if (at >= n) return;
-    if (done) {
-      token = a.eos;
-      total = score;
-    } else {
-      const uint64_t k = in.key[lane][at];
-      token = key_index(k);
-      total = (score + (double)key_value(k)) - lse;  // the sum of two fp32 is exact, or near it
+};
+
+// The W best of the W * S lists, by a whole CTA. W candidates reach the W-th largest
+// of the lists' first ones (of their distinct upper halves); what reaches it is mostly little more than the W, and is
+// ranked by counting (a warp that takes the best head W times over: 450 cycles each).
+__device__ __forceinline__ void merge(Lists& in, const SelectArgs& a, size_t m0, int S,
+                                      const Standing& now) {
+  const int tid = threadIdx.x, W = a.W, lists = W * S;
+  const uint64_t none = order(-(double)INFINITY);
+  if (tid < 32) {
+    const bool on = tid < lists;
+    const double score = canon(now.score);
+    double lse = 0.0;
+    uint64_t head = none;
+    if (on) {
+      if (now.done) {
+        in.n[tid] = tid % S == 0;  // (beam, eos) at its own score
+        head = order(score);
+      } else {
+        const int first = tid - tid % S;
+        float m = in.m[tid];
+        double s = in.s[tid];
+        if (S > 1) {
+#pragma unroll 4
+          for (int i = 0; i < S; ++i) m = fmaxf(m, in.m[first + i]);
+          s = 0.0;
+#pragma unroll 4
+          for (int i = 0; i < S; ++i)
+            s += in.s[first + i] * (double)exp2_fast((in.m[first + i] - m) * LOG2E);
+        }
+        lse = log_sum(m, s);
+        if (in.n[tid]) head = order((score + (double)key_value(in.key[tid][0])) - lse);
+      }
+      in.score[tid] = score;
+      in.lse[tid] = lse;
     }
-    ++at;
+    const uint32_t done = __ballot_sync(~0u, now.done);
+    uint32_t high = (uint32_t)(head >> 32), bound;
+    if (S == 1) {
+      bound = __reduce_min_sync(~0u, on ? high : ~0u);
+    } else {
+      high = on ? high : 0;
+      bound = __reduce_max_sync(~0u, high);
+      for (int j = 1; j < W; ++j) {
+        high = high == bound ? 0 : high;
+        bound = __reduce_max_sync(~0u, high);
+      }
+    }
+    if (tid == 0) in.done = done, in.bound = bound, in.totals = 0;
+  }
+  __syncthreads();
+  for (int c = tid; c < lists * W; c += blockDim.x) {
+    const int list = c / W, i = c % W;
+    if (i >= in.n[list]) continue;
+    // the sum of two fp32 is exact, or near it
+    double t = in.score[list];
+    if (!(in.done >> list & 1)) t = (t + (double)key_value(in.key[list][i])) - in.lse[list];
+    const uint64_t o = order(t);
+    if (o <= none || (uint32_t)(o >> 32) < in.bound) continue;
+    const int at = atomicAdd(&in.totals, 1);
+    in.total[at] = o;
+    in.which[at] = list * 32 + i;
+  }
+  __syncthreads();
+  const int n = in.totals, end = a.eos >= 0 ? a.eos : 0;
+  auto put = [&](int j, float score, int parent, int token, bool done) {
+    a.scores[m0 + j] = score;
+    a.parents[m0 + j] = parent;
+    a.tokens[m0 + j] = token;
+    if (a.finished) a.finished[m0 + j] = done || token == a.eos;
   };
-  next();
-  for (int j = 0; j < W; ++j) {
-    const uint64_t o = order(total);
-    const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(o >> 32));
-    const bool top = (uint32_t)(o >> 32) == hi;
-    const uint32_t lo = __reduce_max_sync(~0u, top ? (uint32_t)o : 0u);
-    const int win = __ffs(__ballot_sync(~0u, top && (uint32_t)o == lo)) - 1;
-    const bool live = __shfl_sync(~0u, total, win) > -INFINITY;
-    const bool stays = __shfl_sync(~0u, done, (j * S) & 31);
-    if (live ? lane == win : lane == 0) {
-      const int t = live ? token : a.eos >= 0 ? a.eos : 0;
-      a.scores[m0 + j] = live ? (float)total : -INFINITY;
-      a.parents[m0 + j] = live ? beam : j;
-      a.tokens[m0 + j] = t;
-      if (a.finished) a.finished[m0 + j] = (live ? done : stays) || t == a.eos;
+  for (int c = tid; c < n; c += blockDim.x) {
+    const uint64_t own = in.total[c];
+    const int which = in.which[c];
+    int place = 0, equal = 0;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const uint64_t t = in.total[k];
+      place += t > own;
+      equal += t == own;
     }
-    if (live && lane == win) next();
+    if (equal > 1)
+      for (int k = 0; k < n; ++k) place += in.total[k] == own && in.which[k] < which;
+    if (place >= W) continue;
+    const int list = which >> 5;
+    const bool done = in.done >> list & 1;
+    put(place, (float)unorder(own), list / S, done ? end : key_index(in.key[list][which & 31]),
+        done);
   }
+  // beams that no candidate is left for
+  for (int j = n + tid; j < W; j += blockDim.x) put(j, -INFINITY, j, end, in.done >> (j * S) & 1);
 }
 
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
@@ -140,6 +194,8 @@ __global__ void __launch_bounds__(32 * ROWS) beam_select_warps_kernel(
   // the first CTA's shared memory may be written once it runs
   const bool many = gridDim.y > 1;
   if (many) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  Standing now;
+  if (blockIdx.y == 0 && warp == 0) now.load(a, m0, 1);
   float m = 0.f;
   double s = 0.0;
   int n = 0;
@@ -155,7 +211,7 @@ __global__ void __launch_bounds__(32 * ROWS) beam_select_warps_kernel(
   if (beam < a.W) deliver(lists, beam, lane, n, keys[warp][lane], m, s);
   if (many) rnet_dev::cluster_sync();
   else __syncthreads();
-  if (blockIdx.y == 0 && warp == 0) merge(lists, a, m0, 1);
+  if (blockIdx.y == 0) merge(lists, a, m0, 1, now);
 }
 
 constexpr int SELECT_CTAS = 16;  // of one sequence's cluster
@@ -180,6 +236,8 @@ __global__ void __launch_bounds__(BeamSelection<T>::NT, 2) beam_select_cluster_k
   // the first CTA's shared memory may be written once it runs
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   bool waited = C == 1;
+  Standing now;
+  if (rank == 0 && tid < 32) now.load(a, m0, S);
   uint32_t parity;
   select_setup(sel, parity);
   for (int u = rank; u < a.W * S; u += C) {
@@ -196,7 +254,7 @@ __global__ void __launch_bounds__(BeamSelection<T>::NT, 2) beam_select_cluster_k
     __syncthreads();  // sel is free again
   }
   if (C > 1) rnet_dev::cluster_sync();
-  if (rank == 0 && tid < 32) merge(lists, a, m0, S);
+  if (rank == 0) merge(lists, a, m0, S, now);
 }
 
 template <class Kernel, class... Args>

@@ -79,8 +79,20 @@ __device__ __forceinline__ float words_sum(const uint32_t* w, float m, float c) 
   return s;
 }
 
-// The r-th largest (r = 1..32) of a warp's 32 values.
+// The r-th largest of the distinct values of a warp that are above -FLT_MAX, or
+// -FLT_MAX: at least r values reach it, or all that are above -FLT_MAX.
+__device__ __forceinline__ float warp_nth_few(float v, int r) {
+  float t = warp_max(v);
+  for (int i = 1; i < r; ++i) {
+    v = v == t ? -FLT_MAX : v;
+    t = warp_max(v);
+  }
+  return t;
+}
+// The r-th largest (r = 1..32) of a warp's 32 values, or, where a few rounds find it
+// sooner, of its distinct values.
 __device__ __forceinline__ float warp_nth(float v, int r) {
+  if (r <= 8) return warp_nth_few(v, r);
   const int lane = threadIdx.x & 31;
   // bitonic sort, largest first
 #pragma unroll
@@ -259,7 +271,8 @@ __device__ __forceinline__ void select_setup(Sel& sel, uint32_t& parity) {
 
 // Leaves the K largest of the n <= SEL_CAP keys, or those of them that `keep`
 // accepts, in any order, and returns a bound that exactly K of all n reach (0 if
-// there are no more than K). All threads, which have read n before.
+// there are no more than K). All threads; a barrier lies between the last key and the
+// call.
 template <class Sel, class Keep>
 __device__ __forceinline__ uint64_t shrink(Sel& sel, int n, int K, Keep keep) {
   constexpr int NT = Sel::NT, J = (SEL_CAP + NT - 1) / NT;
@@ -290,8 +303,8 @@ __device__ __forceinline__ uint64_t shrink(Sel& sel, int n, int K, Keep keep) {
   return t;
 }
 
-// Turns the n queued groups into keys that reach the bound. All threads, which
-// have read n before. Where they are more than there is room for, the bound is
+// Turns the n queued groups into keys that reach the bound, a word to a thread. All
+// threads; a barrier lies between the last group or key and the call. Where they are more than there is room for, the bound is
 // raised to the K-th of those at hand and the groups are gone through again; the
 // keys of earlier groups (elements before `first`) stay.
 template <bool CLEAN, class Sel>
@@ -299,23 +312,22 @@ __device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_
   using T = typename Sel::Type;
   constexpr int N = Sel::N, NT = Sel::NT;
   for (bool again = true; again;) {
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const int word = sel.group_word[i];
+    for (int i = threadIdx.x; i < n * SEL_GROUP; i += NT) {
+      const int g = i / SEL_GROUP, j = i % SEL_GROUP;
+      const int first_of = (sel.group_word[g] + j * NT) * N;
+      const uint32_t w = sel.group[j][g];
 #pragma unroll
-      for (int j = 0; j < SEL_GROUP; ++j)
-#pragma unroll
-        for (int h = 0; h < N; ++h) {
-          const float x = word_value<T, CLEAN>(sel.group[j][i], h);
-          if (!(x > -INFINITY)) continue;
-          const uint64_t k = make_key(x + 0.0f, (word + j * NT) * N + h);
-          if (k < bound) continue;
-          const int at = atomicAdd(&sel.keys, 1);
-          if (at < SEL_CAP) sel.key[at] = k;
-        }
+      for (int h = 0; h < N; ++h) {
+        const float x = word_value<T, CLEAN>(w, h);
+        if (!(x > -INFINITY)) continue;
+        const uint64_t k = make_key(x + 0.0f, first_of + h);
+        if (k < bound) continue;
+        const int at = atomicAdd(&sel.keys, 1);
+        if (at < SEL_CAP) sel.key[at] = k;
+      }
     }
     __syncthreads();
     const int got = sel.keys;
-    __syncthreads();
     again = got > SEL_CAP;
     if (again) {
       const uint64_t t = shrink(sel, SEL_CAP, K, [&](uint64_t k) {
@@ -405,13 +417,14 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
     sum = sum * exp2_fast((m - mx) * c) + words_sum<T, R, CLEAN>(w, mx, c);
     m = mx;
     if (i < 2 || (i & (i - 1)) == 0) {
-      // K logits reach the least of the warps' r-th largest thread maxima so far
+      // K logits reach the K-th largest of the warps' maxima so far, or the least of
+      // their r-th largest thread maxima
       const float v = K <= WARPS ? warp_max(m) : warp_nth(m, (K + WARPS - 1) / WARPS);
       if (lane == 0) sel.bound[i & 1][warp] = v;
       __syncthreads();
-      float least = sel.bound[i & 1][0];
-#pragma unroll
-      for (int j = 1; j < WARPS; ++j) least = fminf(least, sel.bound[i & 1][j]);
+      const bool few = K <= WARPS && K <= 8;
+      const float o = lane < WARPS ? sel.bound[i & 1][lane] : few ? -FLT_MAX : FLT_MAX;
+      const float least = few ? warp_nth_few(o, K) : warp_min(o);
       const uint64_t t = (uint64_t)order(least + 0.0f) << 32;
       if (t > bound) {
         bound = t;
@@ -460,7 +473,6 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
         again = n > SEL_QUEUE;  // then this chunk's groups come again
         drain<CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound);
         const int got = sel.keys, here = w0 * N;
-        __syncthreads();
         const uint64_t t = shrink(sel, got, K, [&](uint64_t k) {
           return !again || key_index(k) < here;
         });
@@ -475,14 +487,8 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
     // the chunk's place is free
     if (tid == 0 && i + SEL_STAGES < chunks && staged(i + SEL_STAGES)) fetch(i + SEL_STAGES);
   }
-  __syncthreads();
-  {
-    const int n = sel.groups;
-    __syncthreads();
-    drain<CLEAN>(sel, n, K, epoch, bound);
-  }
+  drain<CLEAN>(sel, sel.groups, K, epoch, bound);  // complete since the loop's last barrier
   int n = sel.keys;
-  __syncthreads();
   if (n > NT) {
     shrink(sel, n, K, [](uint64_t) { return true; });
     n = sel.keys;
@@ -502,9 +508,7 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
   const double part = warp_sum((double)(sum * exp2_fast((mine - m) * c)));
   if (lane == 0) sel.s[warp] = part;
   __syncthreads();
-  s = 0.0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) s += sel.s[i];
+  s = warp_sum(lane < WARPS ? sel.s[lane] : 0.0);
   return min(n, K);
 }
 template <class Sel, class T>
