@@ -72,11 +72,6 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
   return y;
 }
-__device__ __forceinline__ float warp_min(float v) {
-  float y;
-  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
-  return y;
-}
 // The same as warp_max for groups of G neighbouring lanes.
 template <int G>
 __device__ __forceinline__ float group_max(float v) {

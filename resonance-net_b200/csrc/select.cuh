@@ -79,20 +79,21 @@ __device__ __forceinline__ float words_sum(const uint32_t* w, float m, float c) 
   return s;
 }
 
-// The r-th largest of the distinct values of a warp that are above -FLT_MAX, or
-// -FLT_MAX: at least r values reach it, or all that are above -FLT_MAX.
+// A bound that at least r of a warp's values of type T reach, or all that are above
+// -FLT_MAX, by r rounds: the r-th largest, in fp32, where equal values are rare, of
+// the distinct values.
+template <class T>
 __device__ __forceinline__ float warp_nth_few(float v, int r) {
+  const int lane = threadIdx.x & 31;
   float t = warp_max(v);
   for (int i = 1; i < r; ++i) {
-    v = v == t ? -FLT_MAX : v;
+    if (sizeof(T) == 4 ? v == t : lane == __ffs(__ballot_sync(~0u, v == t)) - 1) v = -FLT_MAX;
     t = warp_max(v);
   }
   return t;
 }
-// The r-th largest (r = 1..32) of a warp's 32 values, or, where a few rounds find it
-// sooner, of its distinct values.
+// The r-th largest (r = 1..32) of a warp's 32 values.
 __device__ __forceinline__ float warp_nth(float v, int r) {
-  if (r <= 8) return warp_nth_few(v, r);
   const int lane = threadIdx.x & 31;
   // bitonic sort, largest first
 #pragma unroll
@@ -146,7 +147,7 @@ __device__ __forceinline__ int warp_select_as(const uint32_t* w, int K, float c,
   // a small one, about the K-th largest of the maxima of the lanes' quarters
   float T_;
   if (K <= 16) {
-    T_ = warp_nth(mine, K);
+    T_ = K <= (N == 1 ? 8 : 4) ? warp_nth_few<T>(mine, K) : warp_nth(mine, K);
   } else {
     constexpr int Q = R / 4;
     uint32_t g[4];
@@ -303,28 +304,29 @@ __device__ __forceinline__ uint64_t shrink(Sel& sel, int n, int K, Keep keep) {
   return t;
 }
 
-// Turns the n queued groups into keys that reach the bound, a word to a thread. All
-// threads; a barrier lies between the last group or key and the call. Where they are more than there is room for, the bound is
+// Turns the n queued groups into keys that reach the bound. All threads; a barrier lies between the last group or key and the call. Where they are more than there is room for, the bound is
 // raised to the K-th of those at hand and the groups are gone through again; the
 // keys of earlier groups (elements before `first`) stay.
 template <bool CLEAN, class Sel>
 __device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_t& bound) {
   using T = typename Sel::Type;
   constexpr int N = Sel::N, NT = Sel::NT;
+  constexpr int EACH = NT < 512 ? SEL_GROUP : 1;  // words of a thread: few threads take a group
   for (bool again = true; again;) {
-    for (int i = threadIdx.x; i < n * SEL_GROUP; i += NT) {
-      const int g = i / SEL_GROUP, j = i % SEL_GROUP;
-      const int first_of = (sel.group_word[g] + j * NT) * N;
-      const uint32_t w = sel.group[j][g];
+    for (int i = threadIdx.x; i < n * (SEL_GROUP / EACH); i += NT) {
+      const int g = i / (SEL_GROUP / EACH), part = i % (SEL_GROUP / EACH) * EACH;
+      const int word = sel.group_word[g];
 #pragma unroll
-      for (int h = 0; h < N; ++h) {
-        const float x = word_value<T, CLEAN>(w, h);
-        if (!(x > -INFINITY)) continue;
-        const uint64_t k = make_key(x + 0.0f, first_of + h);
-        if (k < bound) continue;
-        const int at = atomicAdd(&sel.keys, 1);
-        if (at < SEL_CAP) sel.key[at] = k;
-      }
+      for (int j = part; j < part + EACH; ++j)
+#pragma unroll
+        for (int h = 0; h < N; ++h) {
+          const float x = word_value<T, CLEAN>(sel.group[j][g], h);
+          if (!(x > -INFINITY)) continue;
+          const uint64_t k = make_key(x + 0.0f, (word + j * NT) * N + h);
+          if (k < bound) continue;
+          const int at = atomicAdd(&sel.keys, 1);
+          if (at < SEL_CAP) sel.key[at] = k;
+        }
     }
     __syncthreads();
     const int got = sel.keys;
@@ -422,9 +424,14 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
       const float v = K <= WARPS ? warp_max(m) : warp_nth(m, (K + WARPS - 1) / WARPS);
       if (lane == 0) sel.bound[i & 1][warp] = v;
       __syncthreads();
-      const bool few = K <= WARPS && K <= 8;
-      const float o = lane < WARPS ? sel.bound[i & 1][lane] : few ? -FLT_MAX : FLT_MAX;
-      const float least = few ? warp_nth_few(o, K) : warp_min(o);
+      float least;
+      if (WARPS >= 8 && K <= 8) {
+        least = warp_nth_few<T>(lane < WARPS ? sel.bound[i & 1][lane] : -FLT_MAX, K);
+      } else {
+        least = sel.bound[i & 1][0];
+#pragma unroll
+        for (int j = 1; j < WARPS; ++j) least = fminf(least, sel.bound[i & 1][j]);
+      }
       const uint64_t t = (uint64_t)order(least + 0.0f) << 32;
       if (t > bound) {
         bound = t;
@@ -508,7 +515,9 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
   const double part = warp_sum((double)(sum * exp2_fast((mine - m) * c)));
   if (lane == 0) sel.s[warp] = part;
   __syncthreads();
-  s = warp_sum(lane < WARPS ? sel.s[lane] : 0.0);
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) s += sel.s[i];
   return min(n, K);
 }
 template <class Sel, class T>
