@@ -94,19 +94,22 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // log2 of a softmax term: (x - m) c, c = log2(e) / tau, with the product and
 // the difference in one rounding: the shift is the rounded m c, the same in
-// every term and in the sum, so its rounding cancels. Where m c could leave
-// fp32 (rows whose every logit is masked with the type's lowest value) the
-// difference is taken first.
-__device__ __forceinline__ bool far(float m) { return fabsf(m) > 1e30f; }
+// every term and in the sum, so its rounding cancels. Where that rounding could
+// exceed 1, and 2 to its power leave fp32 (logits far from 0, rows whose every logit
+// is masked with a large number), the difference is taken first: far.
+__device__ __forceinline__ bool far(float m, float c) { return !(fabsf(m * c) < 0x1p24f); }
 __device__ __forceinline__ float term(float x, float m, float c) {
-  return far(m) ? (x - m) * c : fmaf(x, c, -__fmul_rn(m, c));
+  return far(m, c) ? (x - m) * c : fmaf(x, c, -__fmul_rn(m, c));
 }
 // What a sum relative to `from` is multiplied with to be relative to `to`, both
 // the largest logits of parts of a row, from <= to. A part without a logit above
 // -inf has the lowest number as its largest: its sum is 0 (or NaN) and stays so.
 __device__ __forceinline__ float rebase(float from, float to, float c) {
-  const float a = (from - to) * c, b = __fmul_rn(from, c) - __fmul_rn(to, c);
-  return exp2_fast(far(to) ? a : b);
+  const float f = __fmul_rn(from, c), t = __fmul_rn(to, c);
+  float d;
+  if (far(from, c)) d = far(to, c) ? (from - to) * c : fmaf(from, c, -t);
+  else d = far(to, c) ? -fmaf(to, c, -f) : f - t;
+  return exp2_fast(d);
 }
 
 // One 16-byte piece of a row: 4 fp32 or 8 bf16 values.

@@ -312,8 +312,9 @@ struct Share {
     m = fmaxf(piece_max<NP>(x), edge);
     s = s1 = 0.f;
     const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
-    if (far(m)) {
-      fill(x, edge, [&](float v) { return (v - m) * c; }, [&](float v) { return (v - m) * LOG2E; });
+    if (far(m, c) || (HARD && far(m, LOG2E))) {
+      fill(x, edge, [&](float v) { return term(v, m, c); },
+           [&](float v) { return term(v, m, LOG2E); });
     } else {
       fill(x, edge, [&](float v) { return fmaf(v, c, -mc); },
            [&](float v) { return fmaf(v, LOG2E, -m1); });
@@ -354,7 +355,7 @@ struct Share {
     if constexpr (!KEEP) {
       auto at = [&](int i) { return i < E ? x[i / N].get(i % N) : xe; };
       const float mc = __fmul_rn(g.m, g.c), m1 = __fmul_rn(g.m, LOG2E);
-      if (wide && !far(g.m))
+      if (wide && !far(g.m, g.c) && !far(g.m, LOG2E))
         all(true, [&](int i) {
           return fmaf(g.a1, exp2_fast(fmaf(at(i), LOG2E, -m1)),
                       g.a * exp2_fast(fmaf(at(i), g.c, -mc)));
@@ -596,10 +597,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     if (HARD) s1 *= rebase(m, mx, LOG2E);
     m = mx;
     const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
-    if (far(m)) {
+    if (far(m, c) || (HARD && far(m, LOG2E))) {
       each([&](float v) {
-        s += exp2_fast((v - m) * c);
-        if (HARD) s1 += exp2_fast((v - m) * LOG2E);
+        s += exp2_fast(term(v, m, c));
+        if (HARD) s1 += exp2_fast(term(v, m, LOG2E));
       });
     } else {
       each([&](float v) {
@@ -671,7 +672,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     const float e = g.a * exp2_fast(fmaf(v, c, -mc));
     return HARD ? fmaf(g.a1, exp2_fast(fmaf(v, LOG2E, -m1)), e) : e;
   };
-  if (far(m) || ((uintptr_t)p & 15))
+  if (far(m, c) || (HARD && far(m, LOG2E)) || ((uintptr_t)p & 15))
     // also where logits and gradient lie differently on the 16-byte grid
     write(((uintptr_t)p & 15) == 0, [&](float v) { return g.template at<HARD>(v); });
   else

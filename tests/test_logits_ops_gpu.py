@@ -304,6 +304,31 @@ def test_distill_huge_logits_and_extreme_temperatures(rnet, cuda, v, tau):
     _check("f32", got, want)
 
 
+@pytest.mark.parametrize("v", [100, 900, 5000, 40000])
+@pytest.mark.parametrize("tau", [1e-4, 0.3, 1.0, 1e4])
+def test_distill_logits_of_every_magnitude(rnet, cuda, v, tau):
+    """Rows at +-10^e: the rounding of the largest logit over the temperature, far
+    above 1 from 10^8 on, shows in no term."""
+    torch, k = cuda, 4
+    r = np.random.default_rng(v + 1)
+    sizes = [s * 10.0 ** e for e in (3, 5, 7, 8, 9, 10, 12, 17, 25, 29, 31) for s in (1, -1)]
+    n = len(sizes)
+    z = np.zeros((n, v), np.float32)
+    for i, b in enumerate(sizes):
+        # some masked further down, some in another part of the row near the largest
+        z[i] = np.float32(b) + (r.normal(size=v) * 2).astype(np.float32)
+        z[i, v // 3: v // 2] = -np.inf
+        z[i, v // 2: v // 2 + 5] = np.float32(b) * np.float32(1 + 1e-6)
+        z[i, -3:] = np.float32(-3e38)
+    idx = np.tile(np.array([1, v // 2 + 1, 0, -1], np.int32), (n, 1))
+    val = r.normal(size=(n, k)).astype(np.float32)
+    targets = np.full(n, v // 2 + 2, np.int32)
+    _, zz = _place(torch, z, "f32")
+    want = ref.distill(z, idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
+    got = _distill(rnet, torch, zz, "f32", idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
+    _check("f32", got, want)
+
+
 def test_distill_reports_indices_beyond_the_vocabulary(rnet, cuda):
     torch, n, v, k = cuda, 5, 300, 4
     r = np.random.default_rng(1)
