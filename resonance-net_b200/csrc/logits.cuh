@@ -106,9 +106,9 @@ __device__ __forceinline__ float term(float x, float m, float c) {
 // -inf has the lowest number as its largest: its sum is 0 (or NaN) and stays so.
 __device__ __forceinline__ float rebase(float from, float to, float c) {
   const float f = __fmul_rn(from, c), t = __fmul_rn(to, c);
-  float d;
-  if (far(from, c)) d = far(to, c) ? (from - to) * c : fmaf(from, c, -t);
-  else d = far(to, c) ? -fmaf(to, c, -f) : f - t;
+  const float both = (from - to) * c, one = fmaf(from, c, -t), other = -fmaf(to, c, -f);
+  const bool ff = far(from, c), ft = far(to, c);
+  const float d = ff ? (ft ? both : one) : (ft ? other : f - t);
   return exp2_fast(d);
 }
 

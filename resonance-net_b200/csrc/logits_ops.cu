@@ -460,6 +460,7 @@ __device__ __forceinline__ void join_parts(const float4* part, int n, float c, f
   s = s1 = 0.f;
 #pragma unroll
   for (int i = 0; i < MOST; ++i) {
+    if (32 * i >= n) break;
     s += got[i].y * rebase(got[i].x, m, c);
     if (HARD) s1 += got[i].z * rebase(got[i].x, m, LOG2E);
   }
@@ -592,24 +593,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   }
   __syncthreads();  // the barriers are set up
   float m = -FLT_MAX, s = 0.f, s1 = 0.f;
-  auto add = [&](float mx, auto each) {
-    s *= rebase(m, mx, c);
-    if (HARD) s1 *= rebase(m, mx, LOG2E);
-    m = mx;
-    const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
-    if (far(m, c) || (HARD && far(m, LOG2E))) {
-      each([&](float v) {
-        s += exp2_fast(term(v, m, c));
-        if (HARD) s1 += exp2_fast(term(v, m, LOG2E));
-      });
-    } else {
-      each([&](float v) {
-        s += exp2_fast(fmaf(v, c, -mc));
-        if (HARD) s1 += exp2_fast(fmaf(v, LOG2E, -m1));
-      });
+  bool again = false;  // a largest logit on the way was far
+  auto add = [&](float mx, bool first, auto each) {
+    const float mc = __fmul_rn(mx, c), m1 = __fmul_rn(mx, LOG2E);
+    again |= far(mx, c) || (HARD && far(mx, LOG2E));
+    if (!first) {
+      s *= exp2_fast(__fmul_rn(m, c) - mc);
+      if (HARD) s1 *= exp2_fast(__fmul_rn(m, LOG2E) - m1);
     }
+    m = mx;
+    each([&](float v) {
+      s += exp2_fast(fmaf(v, c, -mc));
+      if (HARD) s1 += exp2_fast(fmaf(v, LOG2E, -m1));
+    });
   };
-  if (edge >= 0) add(fmaxf(m, xe), [&](auto f) { f(xe); });
   for (int i = 0; i * CH < n; ++i) {
     // a copy that does not come is reported and given the same time once more:
     // none may land in memory that the CTA has left
@@ -622,12 +619,26 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       x[j].none();
       if (q < n) x[j] = buf[q];
     }
-    add(fmaxf(m, piece_max<4>(x)), [&](auto f) {
+    add(fmaxf(m, piece_max<4>(x)), i == 0, [&](auto f) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int k = 0; k < N; ++k) f(x[j].get(k));
     });
+  }
+  if (edge >= 0) add(fmaxf(m, xe), false, [&](auto f) { f(xe); });
+  if (again) {  // the sums once more, relative to the largest of all
+    s = s1 = 0.f;
+    auto take = [&](float v) {
+      s += exp2_fast(term(v, m, c));
+      if (HARD) s1 += exp2_fast(term(v, m, LOG2E));
+    };
+    for (int q = tid; q < n; q += NT) {
+      const Piece<T> x = buf[q];
+#pragma unroll
+      for (int k = 0; k < N; ++k) take(x.get(k));
+    }
+    if (edge >= 0) take(xe);
   }
   {
     const float mw = warp_max(m);
