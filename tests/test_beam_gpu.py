@@ -111,6 +111,26 @@ def test_many_sequences(rnet, cuda):
     np.testing.assert_array_equal(rk, r0.astype(np.float32))
 
 
+@pytest.mark.parametrize("v", [40, 700, 5000, 40000])
+@pytest.mark.parametrize("batch,beams", [(1, 2), (1, 4), (3, 5), (2, 16), (3, 32)])
+def test_select_uneven_beams(rnet, cuda, v, batch, beams):
+    """One beam that has every choice, one that has none, and finished beams at the
+    top, in the middle and behind: what reaches the merge's bound varies from a few
+    candidates to all of them."""
+    torch, m = cuda, batch * beams
+    r = np.random.default_rng(v + beams)
+    z = _logits(torch, (r.normal(size=(m, v)) * 2.5).astype(np.float32), "f32")
+    steps = np.tile(np.arange(beams), batch)
+    for scores in (-40.0 * steps, 40.0 * steps - 1000.0, -1e4 * (steps == beams - 1) - 0.1 * steps,
+                   -0.01 * steps):
+        scores = (scores - r.random(m) * 1e-2).astype(np.float32)
+        _check_select(rnet, torch, z, "f32", scores, beams)
+        for at in (0, beams // 2, beams - 1):
+            fin = (steps == at).astype(np.int32)
+            _check_select(rnet, torch, z, "f32", scores, beams, eos=v // 2, finished=fin)
+        _check_select(rnet, torch, z, "f32", scores, beams, eos=0, finished=np.ones(m, np.int32))
+
+
 @pytest.mark.parametrize("v", [40, 700, 9000])
 def test_select_first_step_and_masked_rows(rnet, cuda, v):
     torch, beams = cuda, 4
