@@ -136,11 +136,12 @@ _SIGS = {
 }
 
 _lib: Optional[ctypes.CDLL] = None
+_quick = None  # the extension module with quicker entries for some of the functions
 
 
 def lib() -> ctypes.CDLL:
     """Load librnet_b200.so (raises if it has not been built)."""
-    global _lib
+    global _lib, _quick
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} not found: build it with "
@@ -152,6 +153,8 @@ def lib() -> ctypes.CDLL:
             f = getattr(L, name)
             f.argtypes = args
             f.restype = _I
+        from . import _calls
+        _quick = _calls
         _lib = L
     return _lib
 
@@ -166,6 +169,13 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
+    quick = getattr(_quick, name, None)
+    if quick is not None:
+        rc = quick(*args)
+        if rc == 0:
+            return
+        if rc is not NotImplemented:
+            check(rc)
     check(getattr(lib(), name)(*args))
 
 

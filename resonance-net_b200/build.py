@@ -1,7 +1,8 @@
 """Build recipe for librnet_b200.so (sm_100a) — plain nvcc, no CMake.
 
 Every CUDA source under csrc/ and every C++ source under host/ is compiled to
-an object in _build/ and linked into one shared library next to this file.
+an object in _build/ and linked into one shared library next to this file;
+python/calls.cpp becomes the extension module _calls that stands on it.
 Objects are rebuilt when their source or any header in the tree is newer.
 """
 from __future__ import annotations
@@ -11,11 +12,13 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librnet_b200.so")
+CALLS = os.path.join(HERE, "_calls.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -73,7 +76,20 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
+    _build_calls(hdr_mtime)
     return LIB
+
+
+def _build_calls(hdr_mtime: float) -> None:
+    src = os.path.join(HERE, "python", "calls.cpp")
+    if os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), hdr_mtime):
+        return
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I",
+           os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", CALLS,
+           "-L", HERE, "-l:librnet_b200.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building _calls failed:\n" + r.stdout + r.stderr)
 
 
 if __name__ == "__main__":
