@@ -96,18 +96,19 @@ __device__ __forceinline__ float warp_sum(float v) {
 // the difference in one rounding: the shift is the rounded m c, the same in
 // every term and in the sum, so its rounding cancels. Where that rounding could
 // exceed 1, and 2 to its power leave fp32 (logits far from 0, rows whose every logit
-// is masked with a large number), the difference is taken first: far.
-__device__ __forceinline__ bool far(float m, float c) { return !(fabsf(m * c) < 0x1p24f); }
-__device__ __forceinline__ float term(float x, float m, float c) {
-  return far(m, c) ? (x - m) * c : fmaf(x, c, -__fmul_rn(m, c));
+// is masked with a large number), the difference is taken first: from |m| = limit
+// on, which is 2^24 over the largest c in use.
+__device__ __forceinline__ bool far(float m, float limit) { return !(fabsf(m) < limit); }
+__device__ __forceinline__ float term(float x, float m, float c, float limit) {
+  return far(m, limit) ? (x - m) * c : fmaf(x, c, -__fmul_rn(m, c));
 }
 // What a sum relative to `from` is multiplied with to be relative to `to`, both
 // the largest logits of parts of a row, from <= to. A part without a logit above
 // -inf has the lowest number as its largest: its sum is 0 (or NaN) and stays so.
-__device__ __forceinline__ float rebase(float from, float to, float c) {
+__device__ __forceinline__ float rebase(float from, float to, float c, float limit) {
   const float f = __fmul_rn(from, c), t = __fmul_rn(to, c);
   const float both = (from - to) * c, one = fmaf(from, c, -t), other = -fmaf(to, c, -f);
-  const bool ff = far(from, c), ft = far(to, c);
+  const bool ff = far(from, limit), ft = far(to, limit);
   const float d = ff ? (ft ? both : one) : (ft ? other : f - t);
   return exp2_fast(d);
 }

@@ -115,6 +115,7 @@ struct DistillArgs {
   const int* targets;
   const float* weight;
   float inv_tau, tau, soft, hard, scale;
+  float limit;  // of a largest logit that is not far
   float* row_loss;
   unsigned* err;
   int V, K;
@@ -124,12 +125,13 @@ struct DistillArgs {
 struct RowGrad {
   float m;      // largest logit
   float c;      // log2(e) / tau
+  float limit;
   float a, a1;  // factors of 2^term(x, m, c) and of 2^term(x, m, log2(e))
   float pf, hf; // what a unit of teacher probability and the label take off
   template <bool HARD>
   __device__ __forceinline__ float at(float x) const {
-    float v = a * exp2_fast(term(x, m, c));
-    if (HARD) v += a1 * exp2_fast(term(x, m, LOG2E));
+    float v = a * exp2_fast(term(x, m, c, limit));
+    if (HARD) v += a1 * exp2_fast(term(x, m, LOG2E, limit));
     return v;
   }
 };
@@ -210,19 +212,20 @@ struct Record {
   }
   // tau ln(2) term(x, m, c), in the logits' own unit: where the term itself leaves
   // fp32 (a logit masked with the type's lowest value) it is the difference.
-  static __device__ __forceinline__ float unit(float x, float m, float c, float tau) {
-    const float t = term(x, m, c);
+  static __device__ __forceinline__ float unit(float x, float m, float c, float tau,
+                                               float limit) {
+    const float t = term(x, m, c, limit);
     return t == -INFINITY && x > -INFINITY ? x - m : tau * (LN2 * t);
   }
   // This lane's part of tau sum p (ln(2) lp - ln(2) term).
-  __device__ __forceinline__ float kl(float m, float c, float tau) const {
+  __device__ __forceinline__ float kl(float m, float c, float tau, float limit) const {
     float v = 0.f;
 #pragma unroll
     for (int j = 0; j < J; ++j)
       if (p[j] != 0.f) {
-        const float t = term(z[j], m, c);
+        const float t = term(z[j], m, c, limit);
         v += p[j] * (t > -INFINITY ? tau * (LN2 * (lp[j] - t))
-                                   : tau * (LN2 * lp[j]) - unit(z[j], m, c, tau));
+                                   : tau * (LN2 * lp[j]) - unit(z[j], m, c, tau, limit));
       }
     return v;
   }
@@ -235,7 +238,7 @@ struct Record {
       if (P != 0.f) kl += a.tau * (P * (logf(s) - ln));
       l = a.soft * a.tau * kl;
     }
-    if (y >= 0) l += a.hard * (logf(s1) - unit(zy, m, LOG2E, 1.0f));
+    if (y >= 0) l += a.hard * (logf(s1) - unit(zy, m, LOG2E, 1.0f, a.limit));
     return w * l;
   }
   // The record's and the label's elements, those that are `in` this CTA's share,
@@ -290,6 +293,7 @@ __device__ __forceinline__ RowGrad row_factors(float P, bool label, const Distil
   const float gw = none ? 0.f : w * a.scale;
   g.m = m;
   g.c = a.inv_tau * LOG2E;
+  g.limit = a.limit;
   g.pf = a.soft != 0.f ? gw * a.soft * a.tau : 0.f;
   g.hf = label ? gw * a.hard : 0.f;
   g.a = none || a.soft == 0.f ? 0.f : g.pf * __fdividef(P, s);
@@ -308,13 +312,13 @@ struct Share {
   float e[KEEP ? E + 1 : 1], e1[KEEP && HARD ? E + 1 : 1];
   float m, s, s1;  // largest logit and sums, relative to it
 
-  __device__ __forceinline__ void take(const Piece<T>* x, float edge, float c) {
+  __device__ __forceinline__ void take(const Piece<T>* x, float edge, float c,
+                                       float limit) {
     m = fmaxf(piece_max<NP>(x), edge);
     s = s1 = 0.f;
     const float mc = __fmul_rn(m, c), m1 = __fmul_rn(m, LOG2E);
-    if (far(m, c) || (HARD && far(m, LOG2E))) {
-      fill(x, edge, [&](float v) { return term(v, m, c); },
-           [&](float v) { return term(v, m, LOG2E); });
+    if (far(m, limit)) {
+      fill(x, edge, [&](float v) { return (v - m) * c; }, [&](float v) { return (v - m) * LOG2E; });
     } else {
       fill(x, edge, [&](float v) { return fmaf(v, c, -mc); },
            [&](float v) { return fmaf(v, LOG2E, -m1); });
@@ -355,7 +359,7 @@ struct Share {
     if constexpr (!KEEP) {
       auto at = [&](int i) { return i < E ? x[i / N].get(i % N) : xe; };
       const float mc = __fmul_rn(g.m, g.c), m1 = __fmul_rn(g.m, LOG2E);
-      if (wide && !far(g.m, g.c) && !far(g.m, LOG2E))
+      if (wide && !far(g.m, g.limit))
         all(true, [&](int i) {
           return fmaf(g.a1, exp2_fast(fmaf(at(i), LOG2E, -m1)),
                       g.a * exp2_fast(fmaf(at(i), g.c, -mc)));
@@ -425,12 +429,12 @@ __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) dist
   r.gather(z, a.V);
   const float c = a.inv_tau * LOG2E;
   Share<T, E, HARD, true> h;
-  h.take(x, xe, c);
+  h.take(x, xe, c, a.limit);
   r.weigh(row, a, c);
   const float m = group_max<G>(h.m);
-  const float f = rebase(h.m, m, c), f1 = HARD ? rebase(h.m, m, LOG2E) : 0.f;
+  const float f = rebase(h.m, m, c, a.limit), f1 = HARD ? rebase(h.m, m, LOG2E, a.limit) : 0.f;
   const float s = group_sum<G>(h.s * f), s1 = HARD ? group_sum<G>(h.s1 * f1) : 0.f;
-  const float kl = group_sum<G>(r.kl(m, c, a.tau));
+  const float kl = group_sum<G>(r.kl(m, c, a.tau, a.limit));
   if (lane == 0 && on) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   if (!dlogits) return;
@@ -445,8 +449,8 @@ __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) dist
 // A row's maximum and sums from the parts (m, s, s1) of n warps, joined in the
 // same order by every warp.
 template <int MOST, bool HARD>
-__device__ __forceinline__ void join_parts(const float4* part, int n, float c, float& m, float& s,
-                                           float& s1) {
+__device__ __forceinline__ void join_parts(const float4* part, int n, float c, float limit,
+                                           float& m, float& s, float& s1) {
   const int lane = threadIdx.x & 31;
   float4 got[MOST];
   m = -FLT_MAX;
@@ -461,8 +465,8 @@ __device__ __forceinline__ void join_parts(const float4* part, int n, float c, f
 #pragma unroll
   for (int i = 0; i < MOST; ++i) {
     if (32 * i >= n) break;
-    s += got[i].y * rebase(got[i].x, m, c);
-    if (HARD) s1 += got[i].z * rebase(got[i].x, m, LOG2E);
+    s += got[i].y * rebase(got[i].x, m, c, limit);
+    if (HARD) s1 += got[i].z * rebase(got[i].x, m, LOG2E, limit);
   }
   s = warp_sum(s);
   if (HARD) s1 = warp_sum(s1);
@@ -499,25 +503,25 @@ __global__ void __launch_bounds__(256) distill_cta_kernel(const T* logits, long 
   if (warp == 0) r.gather(z, a.V);
   const float c = a.inv_tau * LOG2E;
   Share<T, E, HARD, !HARD> h;
-  h.take(x, xe, c);
+  h.take(x, xe, c, a.limit);
   if (warp == 0) {
     r.weigh(row, a, c);
     if (lane == 0) s_P = r.P, s_label = r.y >= 0;
     if (r.bad && a.err) atomicOr(a.err, rnet_dev::ERR_BAD_INDEX);
   }
   float m = warp_max(h.m);
-  float s = warp_sum(h.s * rebase(h.m, m, c));
-  float s1 = HARD ? warp_sum(h.s1 * rebase(h.m, m, LOG2E)) : 0.f;
+  float s = warp_sum(h.s * rebase(h.m, m, c, a.limit));
+  float s1 = HARD ? warp_sum(h.s1 * rebase(h.m, m, LOG2E, a.limit)) : 0.f;
   if (lane == 0) part[warp] = make_float4(m, s, s1, 0.f);
   __syncthreads();
-  join_parts<1, HARD>(part, 8, c, m, s, s1);
+  join_parts<1, HARD>(part, 8, c, a.limit, m, s, s1);
   if (warp == 0) {
-    const float kl = warp_sum(r.kl(m, c, a.tau));
+    const float kl = warp_sum(r.kl(m, c, a.tau, a.limit));
     if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;
   const RowGrad g = row_factors(s_P, s_label, a, w, m, s, s1);
-  h.write(d, grid, x, xe, tid, 256, grid.pieces, edge, g, HARD ? 0.f : g.a * rebase(h.m, m, c), 0.f);
+  h.write(d, grid, x, xe, tid, 256, grid.pieces, edge, g, HARD ? 0.f : g.a * rebase(h.m, m, c, a.limit), 0.f);
   __syncthreads();  // orders the stores above before those below
   if (warp == 0) r.template fix<HARD>(d, g, a.K, [](int) { return true; });
 }
@@ -596,7 +600,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   bool again = false;  // a largest logit on the way was far
   auto add = [&](float mx, bool first, auto each) {
     const float mc = __fmul_rn(mx, c), m1 = __fmul_rn(mx, LOG2E);
-    again |= far(mx, c) || (HARD && far(mx, LOG2E));
+    again |= far(mx, a.limit);
     if (!first) {
       s *= exp2_fast(__fmul_rn(m, c) - mc);
       if (HARD) s1 *= exp2_fast(__fmul_rn(m, LOG2E) - m1);
@@ -630,8 +634,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   if (again) {  // the sums once more, relative to the largest of all
     s = s1 = 0.f;
     auto take = [&](float v) {
-      s += exp2_fast(term(v, m, c));
-      if (HARD) s1 += exp2_fast(term(v, m, LOG2E));
+      s += exp2_fast(term(v, m, c, a.limit));
+      if (HARD) s1 += exp2_fast(term(v, m, LOG2E, a.limit));
     };
     for (int q = tid; q < n; q += NT) {
       const Piece<T> x = buf[q];
@@ -642,8 +646,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   }
   {
     const float mw = warp_max(m);
-    s = warp_sum(s * rebase(m, mw, c));
-    if (HARD) s1 = warp_sum(s1 * rebase(m, mw, LOG2E));
+    s = warp_sum(s * rebase(m, mw, c, a.limit));
+    if (HARD) s1 = warp_sum(s1 * rebase(m, mw, LOG2E, a.limit));
     m = mw;
   }
   const float4 mine = make_float4(m, s, s1, 0.f);
@@ -660,9 +664,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
     return;
   }
-  join_parts<CLUSTER * NW / 32, HARD>(part, C * NW, c, m, s, s1);
+  join_parts<CLUSTER * NW / 32, HARD>(part, C * NW, c, a.limit, m, s, s1);
   if (rank == 0 && warp == 0) {
-    const float kl = warp_sum(r.kl(m, c, a.tau));
+    const float kl = warp_sum(r.kl(m, c, a.tau, a.limit));
     if (lane == 0) a.row_loss[row] = r.loss(a, w, kl, m, s, s1);
   }
   if (!d) return;
@@ -683,7 +687,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     const float e = g.a * exp2_fast(fmaf(v, c, -mc));
     return HARD ? fmaf(g.a1, exp2_fast(fmaf(v, LOG2E, -m1)), e) : e;
   };
-  if (far(m, c) || (HARD && far(m, LOG2E)) || ((uintptr_t)p & 15))
+  if (far(m, a.limit) || ((uintptr_t)p & 15))
     // also where logits and gradient lie differently on the 16-byte grid
     write(((uintptr_t)p & 15) == 0, [&](float v) { return g.template at<HARD>(v); });
   else
@@ -830,8 +834,9 @@ cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int*
                          const float* weight, float tau, float soft, float hard, float scale,
                          float* row_loss, float* loss, void* dlogits, long long ldd, int rows,
                          int V, int K, unsigned* err, cudaStream_t s) {
-  DistillArgs a{t_idx, t_val, t_lse, targets, weight, 1.0f / tau, tau, soft, hard, scale, row_loss,
-                err, V, K};
+  const float c = LOG2E / tau, most = hard != 0.f && c < LOG2E ? LOG2E : c;
+  DistillArgs a{t_idx, t_val, t_lse, targets, weight,        1.0f / tau, tau, soft,
+                hard,  scale, 0x1p24f / most, row_loss, err, V,          K};
   if (rows > 0) {
     auto run = [&](auto type) {
       using T = decltype(type);

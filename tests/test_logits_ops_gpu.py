@@ -324,9 +324,10 @@ def test_distill_logits_of_every_magnitude(rnet, cuda, v, tau):
     val = r.normal(size=(n, k)).astype(np.float32)
     targets = np.full(n, v // 2 + 2, np.int32)
     _, zz = _place(torch, z, "f32")
-    want = ref.distill(z, idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
-    got = _distill(rnet, torch, zz, "f32", idx, val, tau, 0.6, 0.4, 1.0, targets=targets)
-    _check("f32", got, want)
+    for soft, hard in ((0.6, 0.4), (1.0, 0.0), (0.0, 1.0)):
+        want = ref.distill(z, idx, val, tau, soft, hard, 1.0, targets=targets)
+        got = _distill(rnet, torch, zz, "f32", idx, val, tau, soft, hard, 1.0, targets=targets)
+        _check("f32", got, want)
 
 
 def test_distill_reports_indices_beyond_the_vocabulary(rnet, cuda):
