@@ -41,7 +41,8 @@ int rnet_kernel_launches(unsigned long long* n);
 
 /* Read (and optionally clear) the device error word of the current device:
  * bit 0 = a bounded wait timed out, bit 1 = out-of-range index seen,
- * bit 2 = TMEM allocation failed. Synchronises the device. */
+ * bit 2 = TMEM allocation failed, bit 3 = a selection gave up (its result is
+ * incomplete; not expected on any input). Synchronises the device. */
 int rnet_device_error(unsigned* word, int clear);
 
 /* Self-test of the bounded-wait failure path (no reference counterpart): runs

@@ -19,6 +19,7 @@ enum : unsigned {
   ERR_WAIT_TIMEOUT = 1u << 0,
   ERR_BAD_INDEX = 1u << 1,
   ERR_TMEM_ALLOC = 1u << 2,
+  ERR_NO_PROGRESS = 1u << 3,  // a loop that works towards a bound did not come nearer
 };
 
 // Defined in gemm_tf32x3.cu (one definition per shared library, relocatable

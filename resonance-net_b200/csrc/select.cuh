@@ -304,11 +304,14 @@ __device__ __forceinline__ uint64_t shrink(Sel& sel, int n, int K, Keep keep) {
   return t;
 }
 
-// Turns the n queued groups into keys that reach the bound. All threads; a barrier lies between the last group or key and the call. Where they are more than there is room for, the bound is
-// raised to the K-th of those at hand and the groups are gone through again; the
-// keys of earlier groups (elements before `first`) stay.
+// Turns the n queued groups into keys that reach the bound. All threads; a barrier
+// lies between the last group or key and the call. Where they are more than there is
+// room for, the bound is raised to the K-th of those at hand and the groups are gone
+// through again; the keys of earlier groups (elements before `first`) stay. They are at
+// most K, so that SEL_CAP - K > K keys of these groups are at hand and the bound rises.
 template <bool CLEAN, class Sel>
-__device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_t& bound) {
+__device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_t& bound,
+                                      unsigned* err) {
   using T = typename Sel::Type;
   constexpr int N = Sel::N, NT = Sel::NT;
   constexpr int EACH = NT < 512 ? SEL_GROUP : 1;  // words of a thread: few threads take a group
@@ -335,7 +338,12 @@ __device__ __forceinline__ void drain(Sel& sel, int n, int K, int first, uint64_
       const uint64_t t = shrink(sel, SEL_CAP, K, [&](uint64_t k) {
         return key_index(k) < first;
       });
-      bound = t > bound ? t : bound;
+      if (t <= bound) {  // no round may follow that finds the same keys
+        again = false;
+        if (threadIdx.x == 0 && err) atomicOr(err, rnet_dev::ERR_NO_PROGRESS);
+      } else {
+        bound = t;
+      }
     }
   }
 }
@@ -449,9 +457,12 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
         uint32_t v;
         asm volatile("mov.b32 %0, %1;" : "=r"(v) : "r"(w[g * SEL_GROUP + j]));
 #pragma unroll
-        for (int h = 0; h < N; ++h)
-          in |= make_key(word_value<T, CLEAN>(v, h) + 0.0f,
-                         (w0 + (g * SEL_GROUP + j) * NT + tid) * N + h) >= bound;
+        for (int h = 0; h < N; ++h) {
+          const float x = word_value<T, CLEAN>(v, h);
+          // a NaN gives no key, here as in drain(): it must not bring its group back
+          in |= x > -INFINITY &&
+                make_key(x + 0.0f, (w0 + (g * SEL_GROUP + j) * NT + tid) * N + h) >= bound;
+        }
       }
       return in;
     };
@@ -469,6 +480,9 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
           }
         }
     };
+    // Ends: a group is queued for a key that reaches the bound, so where more are
+    // queued than there is room for, SEL_QUEUE > K keys are at hand, the bound rises to the
+    // K-th, and at most K of those groups come again.
     for (bool again = true; again;) {
       full = false;
       if (!exact) queue([](int) { return true; });
@@ -476,14 +490,19 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
       again = false;
       if (__syncthreads_or(full)) {
         const int n = sel.groups;
+        const uint64_t before = bound;
         __syncthreads();
         again = n > SEL_QUEUE;  // then this chunk's groups come again
-        drain<CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound);
+        drain<CLEAN>(sel, min(n, SEL_QUEUE), K, epoch, bound, err);
         const int got = sel.keys, here = w0 * N;
         const uint64_t t = shrink(sel, got, K, [&](uint64_t k) {
           return !again || key_index(k) < here;
         });
         bound = t > bound ? t : bound;
+        if (again && bound <= before) {
+          again = false;
+          if (tid == 0 && err) atomicOr(err, rnet_dev::ERR_NO_PROGRESS);
+        }
         lowest = key_value(bound);
         exact = true;
         if (tid == 0) sel.groups = 0;
@@ -494,7 +513,7 @@ __device__ __forceinline__ int cta_select_as(Sel& sel, const T* z, int begin, in
     // the chunk's place is free
     if (tid == 0 && i + SEL_STAGES < chunks && staged(i + SEL_STAGES)) fetch(i + SEL_STAGES);
   }
-  drain<CLEAN>(sel, sel.groups, K, epoch, bound);  // complete since the loop's last barrier
+  drain<CLEAN>(sel, sel.groups, K, epoch, bound, err);  // complete since the loop's last barrier
   int n = sel.keys;
   if (n > NT) {
     shrink(sel, n, K, [](uint64_t) { return true; });
