@@ -469,8 +469,10 @@ __global__ void __launch_bounds__(32 * BACK_WARPS) beam_backtrack_kernel(
     }
   }
   if (warp == 0) {
-    const double r =
-        sg.on ? (double)canon(score) / pow((double)len, (double)alpha) : -(double)INFINITY;
+    // 0 and -inf stay what they are: the power may leave 64 bits, and 0 / 0 or inf / inf
+    // would be a rank that is neither above nor below the others
+    double r = sg.on ? (double)canon(score) : -(double)INFINITY;
+    if (r != 0.0 && r != -(double)INFINITY) r /= pow((double)len, (double)alpha);
     int rank = 0;
     for (int i = 0; i < W; ++i) {
       const double o = __shfl_sync(~0u, r, i);
