@@ -1053,6 +1053,12 @@ int Engine::decode_logits(Decoder* d) {
 
 int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
   cudaStream_t s = stream_;
+  if (d->exec && d->graph_precision != precision) {  // the GEMMs' arithmetic is captured
+    cudaGraphExecDestroy(d->exec);
+    cudaGraphDestroy(d->graph);
+    d->exec = nullptr;
+    d->graph = nullptr;
+  }
   if (use_graph && !d->exec) {
     // one eager step first so every kernel attribute / tensor map is set up,
     // then capture the step (all arguments are fixed device pointers; the
@@ -1073,6 +1079,7 @@ int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
     CK(cudaGraphGetNodes(g, nullptr, &nodes));
     d->graph_kernels = (int)nodes;  // the captured step contains kernel nodes only
     CK(cudaGraphInstantiate(&d->exec, g, 0));
+    d->graph_precision = precision;
   }
   for (int i = 0; i < n_steps; ++i) {
     if (d->exec) {
@@ -1143,7 +1150,7 @@ int Engine::beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha
   Decoder::Beam& b = d->beam;
   const int groups = d->M / beams;
   cudaStream_t s = stream_;
-  if (b.exec && (b.beams != beams || b.eos != eos)) {
+  if (b.exec && (b.beams != beams || b.eos != eos || b.precision != precision)) {
     cudaGraphExecDestroy(b.exec);
     b.exec = nullptr;
   }
@@ -1171,6 +1178,7 @@ int Engine::beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha
       b.kernels = (int)nodes;  // kernel nodes only
       b.beams = beams;
       b.eos = eos;
+      b.precision = precision;
     }
     if (use_graph && b.exec) {
       CK(cudaGraphLaunch(b.exec, s));

@@ -87,6 +87,7 @@ struct Decoder {
   cudaGraphExec_t exec = nullptr;
   cudaGraph_t graph = nullptr;
   int graph_kernels = 0;
+  int graph_precision = 0;  // of the captured step's GEMMs
   // next-token rule: greedy when temperature <= 0, else temperature + top-p
   // sampling (src/main.cpp:327-360) with a counter-based uniform per
   // (seed, stream, position)
@@ -103,7 +104,7 @@ struct Decoder {
     int cap = 0;
     // the captured step and what it holds
     cudaGraphExec_t exec = nullptr;
-    int beams = 0, eos = 0, kernels = 0;
+    int beams = 0, eos = 0, precision = 0, kernels = 0;
   } beam;
 };
 
