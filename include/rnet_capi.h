@@ -413,8 +413,7 @@ int rnet_decoder_prefill(rnet_decoder* d, const int* d_tokens, int seq_len);
 /* Prefill for a beam search: d_tokens [n_streams / beams, seq_len], one prompt
  * per sequence; its `beams` streams (in a row) all start from its state. */
 int rnet_decoder_prefill_beams(rnet_decoder* d, const int* d_tokens, int seq_len, int beams);
-/* Beam search of n_steps tokens from the current logits and states (after a
- * prefill): n_streams / beams sequences of `beams` streams each, beams 1..32
+/* Beam search of n_steps tokens from the current logits and states: n_streams / beams sequences of `beams` streams each, beams 1..32
  * dividing n_streams; a sequence starts from its first stream. Per step:
  * rnet_beam_select on the logits, rnet_beam_reorder of the recurrent states by
  * the parents, one decode step. eos = -1: no token ends a beam. Outputs (device)
@@ -423,7 +422,9 @@ int rnet_decoder_prefill_beams(rnet_decoder* d, const int* d_tokens, int seq_len
  * score / length^length_alpha. use_graph = 1 replays one captured CUDA graph per
  * step. Asynchronous on the model stream, except that it waits when the record
  * of steps has to grow. Afterwards the streams hold the beams of the last
- * selection, unranked, and rnet_decoder_step(d, NULL) feeds their last tokens. */
+ * selection, unranked, and rnet_decoder_step(d, NULL) feeds their last tokens; the
+ * logits are still those that the last selection chose from. A search without a
+ * prefill, step or generation since the last one is refused (RNET_ERR_ARG). */
 int rnet_decoder_beam_search(rnet_decoder* d, int beams, int n_steps, int eos, float length_alpha,
                              int* d_sequences, int* d_lengths, float* d_scores, int use_graph);
 /* One token per stream: d_tokens [n_streams] (device) or NULL to feed back

@@ -927,6 +927,7 @@ int Engine::prefill(Decoder* d, const int* d_tokens, int T, int copies) {
   const int M = d->M, rows = M / copies, N = rows * T, D = cfg_.d_model, V = cfg_.vocab_size;
   int rc = ensure_capacity(N, false);
   if (rc) return rc;
+  d->current = false;
   cudaStream_t s = stream_;
   unsigned* err = rnet_status::device_error_word();
   const size_t ND = (size_t)N * D;
@@ -957,6 +958,7 @@ int Engine::prefill(Decoder* d, const int* d_tokens, int T, int copies) {
   CK(cudaStreamSynchronize(s));  // &T is a stack value
   CK(rnet_k::sample_rows(d->logits, M, V, d->temperature, d->top_p, d->seed, d->tok, d->pos, 0,
                          s));
+  d->current = true;
   return RNET_OK;
 }
 
@@ -968,6 +970,7 @@ int Engine::decode_step(Decoder* d, const int* d_tokens) {
   if (rc) return rc;
   CK(rnet_k::sample_rows(d->logits, d->M, cfg_.vocab_size, d->temperature, d->top_p, d->seed,
                          d->tok, d->pos, 1, s));
+  d->current = true;
   return RNET_OK;
 }
 
@@ -1085,6 +1088,7 @@ int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
     if (d->exec) {
       CK(cudaGraphLaunch(d->exec, s));
       rnet_status::count_launch((unsigned)d->graph_kernels);
+      d->current = true;
     } else {
       int rc = decode_step(d, nullptr);
       if (rc) return rc;
@@ -1145,8 +1149,12 @@ int Engine::beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha
     return rnet_status::fail(RNET_ERR_ARG, "beam_search: n_streams must be a multiple of beams");
   if (d->M / beams > 65535)
     return rnet_status::fail(RNET_ERR_UNSUPPORTED, "beam_search: more than 65535 sequences");
+  if (!d->current)
+    return rnet_status::fail(RNET_ERR_ARG,
+                             "beam_search: no logits of the streams' last tokens: prefill or step first");
   int rc = beam_reserve(d, n_steps);
   if (rc) return rc;
+  d->current = false;  // the last selection is not stepped on
   Decoder::Beam& b = d->beam;
   const int groups = d->M / beams;
   cudaStream_t s = stream_;

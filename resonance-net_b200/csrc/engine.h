@@ -83,6 +83,9 @@ struct Decoder {
   float* w;
   int* tok;  // current / next token per stream
   int* pos;  // device scalar: index of the token being processed
+  // logits follow the streams' last tokens: after a prefill or step, until a beam
+  // search has chosen from them
+  bool current = false;
   void* arena = nullptr;
   cudaGraphExec_t exec = nullptr;
   cudaGraph_t graph = nullptr;
