@@ -401,7 +401,7 @@ int rnet_model_profile_read(rnet_model* m, double* ms, double* flops, double* by
  * causal-conv inputs and the MinGRU h; 15 * d_model floats per layer per
  * stream). n_streams advance in lock step. The reference has no counterpart
  * (its `generate()` is declared, never defined; `infer` recomputes the whole
- * prefix per token). */
+ * prefix per token). A decoder is destroyed before its model. */
 typedef struct rnet_decoder rnet_decoder;
 int rnet_decoder_create(rnet_model* m, int n_streams, rnet_decoder** out);
 int rnet_decoder_destroy(rnet_decoder* d);

@@ -201,6 +201,7 @@ class Model:
     def __init__(self, cfg: ModelConfig, device: int = 0, reference_init: bool = True,
                  _handle: Optional[int] = None):
         self._h = _P()
+        self._decoders: list[_P] = []  # handles that stand on this model
         if _handle is not None:
             self._h = _P(_handle)
         else:
@@ -220,6 +221,11 @@ class Model:
         return cls(None, _handle=h.value)
 
     def close(self) -> None:
+        # the decoders first: a collected cycle finalises its objects in any order
+        while self._decoders:
+            h = self._decoders.pop()
+            lib().rnet_decoder_destroy(h)
+            h.value = None
         if self._h:
             lib().rnet_model_destroy(self._h)
             self._h = _P()
@@ -360,13 +366,14 @@ class Model:
 
 
 class Decoder:
-    """Batched recurrent decoder over a Model (n_streams in lock step)."""
+    """Batched recurrent decoder over a Model (n_streams in lock step); closed with it."""
 
     def __init__(self, model: Model, n_streams: int):
         self.model = model
         self.M = n_streams
         self.handle = _P()
         check(lib().rnet_decoder_create(model.handle, n_streams, ctypes.byref(self.handle)))
+        model._decoders.append(self.handle)
 
     def prefill(self, d_tokens, seq_len: int) -> None:
         check(lib().rnet_decoder_prefill(self.handle, _ptr(d_tokens), seq_len))
@@ -413,6 +420,7 @@ class Decoder:
 
     def close(self) -> None:
         if self.handle:
+            self.model._decoders = [h for h in self.model._decoders if h is not self.handle]
             lib().rnet_decoder_destroy(self.handle)
             self.handle = _P()
 
