@@ -153,8 +153,11 @@ def lib() -> ctypes.CDLL:
             f = getattr(L, name)
             f.argtypes = args
             f.restype = _I
-        from . import _calls
-        _quick = _calls
+        try:
+            from . import _calls
+            _quick = _calls
+        except ImportError:  # not built for this interpreter: calls go through ctypes
+            _quick = None
         _lib = L
     return _lib
 

@@ -2,8 +2,9 @@
 
 Every CUDA source under csrc/ and every C++ source under host/ is compiled to
 an object in _build/ and linked into one shared library next to this file;
-python/calls.cpp becomes the extension module _calls that stands on it.
-Objects are rebuilt when their source or any header in the tree is newer.
+python/calls.cpp becomes the extension module _calls that stands on it, where
+Python's headers are there (the binding does without it). Objects are rebuilt
+when their source or any header in the tree is newer.
 """
 from __future__ import annotations
 
@@ -18,7 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librnet_b200.so")
-CALLS = os.path.join(HERE, "_calls.so")
+# named for the interpreter: another one neither loads it nor takes it for its own
+CALLS = os.path.join(HERE, "_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -82,14 +84,23 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
 
 def _build_calls(hdr_mtime: float) -> None:
     src = os.path.join(HERE, "python", "calls.cpp")
+    untagged = os.path.join(HERE, "_calls.so")  # an earlier name, which any interpreter finds
+    if CALLS != untagged and os.path.exists(untagged):
+        os.remove(untagged)
     if os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), hdr_mtime):
         return
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I",
            os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", CALLS,
            "-L", HERE, "-l:librnet_b200.so", "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("building _calls failed:\n" + r.stdout + r.stderr)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        failed = r.stdout + r.stderr if r.returncode else None
+    except OSError as e:
+        failed = str(e)
+    if failed is not None:
+        if os.path.exists(CALLS):  # made for other headers: its calls may not fit
+            os.remove(CALLS)
+        sys.stderr.write("_calls was not built, calls go through ctypes:\n" + failed + "\n")
 
 
 if __name__ == "__main__":
