@@ -218,8 +218,10 @@ int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const
  * 1..32. (No counterpart in the reference.)
  *
  * One selection: per sequence, the `beams` candidates (b, v) with the largest
- * scores_in[b] + log softmax(logits[b])[v], sorted, ties to the lowest
- * b * vocab + v. Totals are compared in 64 bits. finished_in[b] != 0 (NULL =
+ * scores_in[b] + log softmax(logits[b])[v], sorted. Totals are formed and compared in
+ * 64 bits; equal ones go to the lower beam, then the larger logit, then the lower
+ * token (a score may be so large, or logits so small, that unequal logits give equal
+ * totals). A chosen total beyond fp32 is stored as infinity. finished_in[b] != 0 (NULL =
  * none finished; needs eos >= 0): the beam has ended and offers only
  * (b, eos) at its own score. Outputs [batch * beams]: scores, tokens, parents
  * (the beam 0..beams-1 each one continues) and finished (may be NULL without

@@ -35,7 +35,7 @@ struct Lists {
   int n[RNET_BEAMS_MAX];
   // the merge's own
   uint64_t total[RNET_BEAMS_MAX * RNET_BEAMS_MAX];
-  int which[RNET_BEAMS_MAX * RNET_BEAMS_MAX];  // 32 list + place: the order of equal totals
+  int which[RNET_BEAMS_MAX * RNET_BEAMS_MAX];  // 32 list + place
   double score[RNET_BEAMS_MAX], lse[RNET_BEAMS_MAX];
   uint32_t done, bound;
   int totals;
@@ -143,10 +143,18 @@ __device__ __forceinline__ void merge(Lists& in, const SelectArgs& a, size_t m0,
       place += t > own;
       equal += t == own;
     }
-    if (equal > 1)
-      for (int k = 0; k < n; ++k) place += in.total[k] == own && in.which[k] < which;
-    if (place >= W) continue;
     const int list = which >> 5;
+    if (equal > 1) {
+      // the lower beam, then the larger logit or lower token: a row's slices do not show
+      const uint64_t key = in.key[list][which & 31];
+      for (int k = 0; k < n; ++k) {
+        const int other = in.which[k] >> 5, beam = other / S;
+        place += in.total[k] == own &&
+                 (beam < list / S ||
+                  (beam == list / S && in.key[other][in.which[k] & 31] > key));
+      }
+    }
+    if (place >= W) continue;
     const bool done = in.done >> list & 1;
     put(place, (float)unorder(own), list / S, done ? end : key_index(in.key[list][which & 31]),
         done);

@@ -182,8 +182,8 @@ cudaError_t distill_topk(const void* logits, bool bf16, long long ld, const int*
 
 // ---- beam search (beam.cu) --------------------------------------------------
 // Per sequence, the `beams` best of score[b] + log softmax(logits[b])[v] over
-// (b, v), ties to the lowest b * V + v; a finished beam offers (b, eos) at its
-// own score only. Outputs may be the inputs of the same name.
+// (b, v), equal totals to the lower beam, larger logit, lower token; a finished
+// beam offers (b, eos) at its own score only. Outputs may be the inputs of the same name.
 cudaError_t beam_select(const void* logits, bool bf16, long long ld, const float* scores_in,
                         const int* finished_in, int eos, float* scores, int* tokens, int* parents,
                         int* finished, int batch, int beams, int V, unsigned* err, cudaStream_t s);
