@@ -1,6 +1,7 @@
 // Beam search: selection over beams and vocabulary, reordering of the streams'
 // states by the chosen parents, and the sequences behind the last beams.
 #include "common.cuh"
+#include "gemm.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
 #include "select.cuh"
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(32 * ROWS) beam_select_warps_kernel(
   if (blockIdx.y == 0) merge(lists, a, m0, 1, now);
 }
 
-constexpr int SELECT_CTAS = 16;  // of one sequence's cluster
+constexpr int SELECT_CTAS = 16;  // of one sequence's cluster, where the device places them
 
 // Two CTAs of 512 threads to an SM hide each other's latency better than more
 // values to a thread (32 x 8 rows of 50001 fp32 in L2: 21.1 us with 256 threads of
@@ -269,18 +270,8 @@ __global__ void __launch_bounds__(BeamSelection<T>::NT, 2) beam_select_cluster_k
 template <class Kernel, class... Args>
 cudaError_t launch_cluster(Kernel kernel, int batch, int C, int threads, size_t smem,
                            cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(batch, C);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.y = C;
-  at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  const ClusterLaunch l(dim3(batch, C), threads, smem, s);
+  return cudaLaunchKernelEx(&l.cfg, kernel, args...);
 }
 
 template <class T>
@@ -294,19 +285,24 @@ cudaError_t select_launch(const T* z, long long ld, const SelectArgs& a, int bat
                                 : beam_select_warps_kernel<T, 64 / N>;
     return launch_cluster(kernel, batch, C, threads, 0, s, z, ld, a);
   }
+  auto kernel = beam_select_cluster_kernel<T>;
+  constexpr int smem = sizeof(BeamSelection<T>);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem((const void*)kernel, smem, ready);
+  if (e != cudaSuccess) return e;
+  static std::atomic<int> known[64];
+  int most;
+  e = cluster_ctas((const void*)kernel, SELECT_CTAS, BeamSelection<T>::NT, smem, known, most);
+  if (e != cudaSuccess) return e;
   // slices of a row where the rows alone leave SMs idle, a chunk or more each
+  const int sms = rnet_gemm::num_sms();
   int S = 1;
-  while (a.W * (S + 1) <= SELECT_CTAS && (long long)batch * a.W * (S + 1) <= 148 &&
+  while (a.W * (S + 1) <= most && (long long)batch * a.W * (S + 1) <= sms &&
          S * BeamSelection<T>::CHUNK * N < a.V)
     ++S;
   const int slice = (((a.V + S - 1) / S) + 15) & ~15;  // whole 16-byte places
-  const int C = a.W * S < SELECT_CTAS ? a.W * S : SELECT_CTAS;
-  auto kernel = beam_select_cluster_kernel<T>;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem((const void*)kernel, sizeof(BeamSelection<T>), ready, true);
-  if (e != cudaSuccess) return e;
-  return launch_cluster(kernel, batch, C, BeamSelection<T>::NT, sizeof(BeamSelection<T>), s, z, ld,
-                        a, S, slice);
+  const int C = a.W * S < most ? a.W * S : most;
+  return launch_cluster(kernel, batch, C, BeamSelection<T>::NT, smem, s, z, ld, a, S, slice);
 }
 
 // ---------------------------------------------------------------- states
@@ -609,7 +605,7 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
   const int per_warp = 32 / P;
   int warps = (steps + BACK * per_warp - 1) / (BACK * per_warp);
   int ctas = 1;
-  while (ctas < BACK_CTAS && warps > 8 * ctas && (long long)batch * 2 * ctas <= 148) ctas *= 2;
+  while (ctas < BACK_CTAS && warps > 8 * ctas && (long long)batch * 2 * ctas <= rnet_gemm::num_sms()) ctas *= 2;
   warps = (warps + ctas - 1) / ctas;
   if (warps > BACK_WARPS) warps = BACK_WARPS;
   const int segments = ctas * warps * per_warp;

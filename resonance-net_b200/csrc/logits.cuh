@@ -13,20 +13,55 @@
 
 namespace rnet_logits {
 
-// Lets a kernel use `bytes` of dynamic shared memory on the current device, and
-// clusters of more than 8 CTAs if it wants them, once per device: `ready` is the
-// kernel's own record of devices.
-inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready,
-                              bool large_clusters = false) {
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once per
+// device: `ready` is the kernel's own record of devices.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 64 && (ready.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && large_clusters)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
+}
+
+// Launch of `grid` CTAs in clusters of grid.y.
+struct ClusterLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  ClusterLaunch(dim3 grid, int threads, size_t smem, cudaStream_t s) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.y = grid.y;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = grid.y > 1;
+  }
+};
+
+// How many CTAs of a kernel may form a cluster: `wanted` (above 8, which every device
+// places) where the current device, or the part of it that the process has, can place
+// them, else 8. Asked once per device: `known` holds the answers.
+inline cudaError_t cluster_ctas(const void* kernel, int wanted, int threads, size_t smem,
+                                std::atomic<int> (&known)[64], int& ctas) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (ctas = known[dev].load(std::memory_order_relaxed))) return cudaSuccess;
+  ctas = 8;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  int fit = 0;
+  ClusterLaunch one(dim3(1, wanted), threads, smem, nullptr);
+  if (cudaOccupancyMaxActiveClusters(&fit, kernel, &one.cfg) != cudaSuccess)
+    cudaGetLastError();  // not placed: no error of this call
+  else if (fit > 0)
+    ctas = wanted;
+  if (dev < 64) known[dev].store(ctas, std::memory_order_relaxed);
+  return cudaSuccess;
 }
 
 __device__ __forceinline__ float to_f(float x) { return x; }

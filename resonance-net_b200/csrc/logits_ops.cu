@@ -1,6 +1,7 @@
 // Records of a row's largest logits, and the distillation loss against such
 // records with its gradient.
 #include "common.cuh"
+#include "gemm.cuh"
 #include "kernels.cuh"
 #include "logits.cuh"
 #include "select.cuh"
@@ -96,7 +97,8 @@ cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, c
     // while every row has an SM of its own, more threads for it (148 rows of 50001
     // fp32, top 64: 16.0 us with 512 threads, 26.9 with 128; 592 rows: 35.7 with 128;
     // 256 threads lie between)
-    return rows <= 148 ? topk_cta<T, 512>(z, ld, a, rows, s) : topk_cta<T, 128>(z, ld, a, rows, s);
+    return rows <= rnet_gemm::num_sms() ? topk_cta<T, 512>(z, ld, a, rows, s)
+                                        : topk_cta<T, 128>(z, ld, a, rows, s);
   return cudaGetLastError();
 }
 
@@ -714,32 +716,22 @@ cudaError_t distill_long_as(const T* z, long long ld, T* d, long long ldd, const
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem((const void*)kernel, 16 * CHUNK<NT> * CHUNKS, ready);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows, C);
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = (size_t)per * 16;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.y = C;
-  at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1;
-  return cudaLaunchKernelEx(&cfg, kernel, z, ld, d, ldd, a, per);
+  const ClusterLaunch l(dim3(rows, C), NT, (size_t)per * 16, s);
+  return cudaLaunchKernelEx(&l.cfg, kernel, z, ld, d, ldd, a, per);
 }
 
 template <class T, int J, bool HARD>
 cudaError_t distill_long(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                          int rows, cudaStream_t s) {
-  const int pieces = a.V / Piece<T>::N;
+  const int pieces = a.V / Piece<T>::N, sms = rnet_gemm::num_sms();
   // one CTA while the row fits one, else shares of the smaller size (2048 rows of
   // 30000 fp32: 90.5 us in three CTAs, 106 in two)
   int C = pieces <= SHARE ? 1 : (pieces + SHARE_256 - 1) / SHARE_256;
   if (C > CLUSTER) C = (pieces + SHARE - 1) / SHARE;
   // more CTAs while they would leave SMs idle and have two chunks each
-  while (C < CLUSTER && (long long)rows * (C + 1) <= 148 && pieces / (C + 1) >= 1024) ++C;
+  while (C < CLUSTER && (long long)rows * (C + 1) <= sms && pieces / (C + 1) >= 1024) ++C;
   if (C > CLUSTER) C = CLUSTER;
-  return (pieces + C - 1) / C <= SHARE_256 && rows > 148
+  return (pieces + C - 1) / C <= SHARE_256 && rows > sms
              ? distill_long_as<T, 256, J, HARD>(z, ld, d, ldd, a, rows, C, s)
              : distill_long_as<T, 512, J, HARD>(z, ld, d, ldd, a, rows, C, s);
 }
