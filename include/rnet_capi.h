@@ -251,9 +251,9 @@ int rnet_beam_reorder(const void* src, void* dst, size_t row_bytes, size_t row_p
  * beams] the last one's. sequences [batch * beams, n_steps]: per sequence the
  * beams sorted by score / length^length_alpha (64 bits, ties to the lower
  * beam; any finite length_alpha, and a score of 0 or -inf stays as it is; NaN counts
- * as -inf, +inf as the largest finite fp32); length counts the tokens up to and including the first eos (n_steps
- * without one, or with eos < 0), and eos fills what follows. lengths and
- * ranked_scores [batch * beams] are in the same order (ranked_scores may be
+ * as -inf, +inf as the largest finite fp32); length counts the tokens up to and
+ * including the first eos (n_steps without one, or with eos < 0), and eos fills
+ * what follows. lengths and ranked_scores [batch * beams] are in the same order (ranked_scores may be
  * scores). A parent outside 0..beams-1 counts as the beam itself and sets the
  * device error word (bit 1). */
 int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
@@ -415,11 +415,12 @@ int rnet_decoder_prefill(rnet_decoder* d, const int* d_tokens, int seq_len);
 /* Prefill for a beam search: d_tokens [n_streams / beams, seq_len], one prompt
  * per sequence; its `beams` streams (in a row) all start from its state. */
 int rnet_decoder_prefill_beams(rnet_decoder* d, const int* d_tokens, int seq_len, int beams);
-/* Beam search of n_steps tokens from the current logits and states: n_streams / beams sequences of `beams` streams each, beams 1..32
- * dividing n_streams; a sequence starts from its first stream. Per step:
- * rnet_beam_select on the logits, rnet_beam_reorder of the recurrent states by
- * the parents, one decode step. eos = -1: no token ends a beam. Outputs (device)
- * as rnet_beam_backtrack with n_steps: d_sequences [n_streams, n_steps],
+/* Beam search of n_steps (1..2^30) tokens from the current logits and states:
+ * n_streams / beams sequences of `beams` streams each, beams 1..32 dividing
+ * n_streams; a sequence starts from its first stream. Per step: rnet_beam_select
+ * on the logits, rnet_beam_reorder of the recurrent states by the parents, one
+ * decode step. eos = -1: no token ends a beam. Outputs (device) as
+ * rnet_beam_backtrack with n_steps: d_sequences [n_streams, n_steps],
  * d_lengths and d_scores [n_streams], ranked per sequence by
  * score / length^length_alpha. use_graph = 1 replays one captured CUDA graph per
  * step. Asynchronous on the model stream, except that it waits when the record

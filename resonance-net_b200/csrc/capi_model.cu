@@ -340,7 +340,8 @@ int rnet_decoder_beam_search(rnet_decoder* d, int beams, int n_steps, int eos, f
   if (beams < 1 || beams > RNET_BEAMS_MAX)
     return rnet_status::fail(RNET_ERR_ARG, "beam_search: beams must be 1.." +
                                                std::to_string(RNET_BEAMS_MAX));
-  if (n_steps < 1) return rnet_status::fail(RNET_ERR_ARG, "beam_search: n_steps must be >= 1");
+  if (n_steps < 1 || n_steps > (1 << 30))
+    return rnet_status::fail(RNET_ERR_ARG, "beam_search: n_steps must be 1..2^30");
   if (eos < -1 || eos >= d->m->e->config().vocab_size)
     return rnet_status::fail(RNET_ERR_ARG, "beam_search: eos must be -1 (none) or a token");
   if (!std::isfinite(length_alpha))
