@@ -86,7 +86,7 @@ cudaError_t topk_cta(const T* z, long long ld, const TopkArgs& a, int rows, cuda
 template <class T>
 cudaError_t topk_launch(const T* z, long long ld, const TopkArgs& a, int rows, cudaStream_t s) {
   constexpr int N = Words<T>::N;
-  const int grid = (rows + TOPK_WARPS - 1) / TOPK_WARPS, block = 32 * TOPK_WARPS;
+  const int grid = (rows - 1) / TOPK_WARPS + 1, block = 32 * TOPK_WARPS;
   if (a.V <= 256)
     topk_warp_kernel<T, 8 / N><<<grid, block, 0, s>>>(z, ld, a, rows);
   else if (a.V <= 1024)
@@ -741,7 +741,7 @@ void distill_warp(const T* z, long long ld, T* d, long long ldd, const DistillAr
                   cudaStream_t s) {
   constexpr int PER = WARPS * (32 / G);  // rows of a CTA
   distill_warp_kernel<T, E, G, J, HARD>
-      <<<(rows + PER - 1) / PER, 32 * WARPS, 0, s>>>(z, ld, d, ldd, a, rows);
+      <<<(rows - 1) / PER + 1, 32 * WARPS, 0, s>>>(z, ld, d, ldd, a, rows);
 }
 
 template <class T, int J, bool HARD>
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* __restrict_
   rnet_dev::pdl_wait();
   rnet_dev::pdl_trigger();
   double a = 0.0;
-  int i = threadIdx.x;
+  long long i = threadIdx.x;  // steps past the last of up to 2^31 - 1 rows
   for (; i + 7 * 1024 < n; i += 8 * 1024) {
     float v[8];
 #pragma unroll
