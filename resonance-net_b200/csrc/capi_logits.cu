@@ -22,6 +22,9 @@ bool aligned(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
 
 size_t elem(int dtype) { return dtype == RNET_DTYPE_BF16 ? 2 : 4; }
 
+// Whether the bytes up to the last of `rows` rows can be counted.
+bool pitch_fits(int rows, long long ld) { return rows == 0 || ld <= (1LL << 60) / rows; }
+
 // Bytes that `rows` rows with a pitch of ld elements span.
 size_t span(int rows, long long ld, int vocab, int dtype) {
   return rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)vocab) * elem(dtype) : 0;
@@ -48,6 +51,7 @@ int rnet_topk_logits_forward(const void* logits, int dtype, long long ld, float 
   NEED(rows >= 0 && vocab > 0, "topk_logits_forward: bad size");
   NEED(vocab <= RNET_SELECT_VOCAB_MAX, "topk_logits_forward: vocab above 2^30");
   NEED(ld >= vocab, "topk_logits_forward: row pitch below vocab");
+  NEED(pitch_fits(rows, ld), "topk_logits_forward: row pitch too large");
   NEED(top_k >= 1 && top_k <= RNET_TOPK_MAX && top_k <= vocab,
        "topk_logits_forward: " + TOPK_RANGE + " and not above vocab");
   NEED(temperature >= 1e-4f && temperature <= 1e4f,
@@ -72,7 +76,7 @@ int rnet_distill_topk_forward(const void* logits, int dtype, long long ld, const
   NEED(rows >= 0 && vocab > 0, "distill_topk_forward: bad size");
   NEED(ld >= vocab && (!dlogits || ld_dlogits >= vocab),
        "distill_topk_forward: row pitch below vocab");
-  NEED(rows == 0 || (ld <= (1LL << 60) / rows && (!dlogits || ld_dlogits <= (1LL << 60) / rows)),
+  NEED(pitch_fits(rows, ld) && (!dlogits || pitch_fits(rows, ld_dlogits)),
        "distill_topk_forward: row pitch too large");
   if (vocab > RNET_DISTILL_VOCAB_MAX)
     return rnet_status::fail(RNET_ERR_UNSUPPORTED,
@@ -110,6 +114,7 @@ int rnet_beam_select(const void* logits, int dtype, long long ld, const float* s
   NEED((long long)batch * beams <= 0x7fffffffLL, "beam_select: batch * beams too large");
   NEED(vocab <= RNET_SELECT_VOCAB_MAX, "beam_select: vocab above 2^30");
   NEED(ld >= vocab, "beam_select: row pitch below vocab");
+  NEED(pitch_fits(batch * beams, ld), "beam_select: row pitch too large");
   NEED(eos >= -1 && eos < vocab, "beam_select: eos must be -1 (none) or a token");
   NEED(!finished_in || (eos >= 0 && finished),
        "beam_select: finished beams need an eos token and the finished output");
