@@ -1,4 +1,4 @@
-"""As many rows as an int counts. Rows of one logit: about 36 GB."""
+"""As many rows as an int counts (rows of one logit, about 36 GB), and the longest row."""
 import math
 
 import pytest
@@ -47,3 +47,28 @@ def test_records(rnet, room):
               idx.data_ptr(), None, n, 1, 1, None)
     torch.cuda.synchronize()
     assert torch.all(idx == 0) and torch.all(top[:n - 1] == 1.5) and float(top[n - 1]) == 2.0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_largest_vocabulary(rnet, room, dtype):
+    """A row of 2^30 logits. A thread adds a partial sum for each of 65536 chunks."""
+    torch, v, k = room, 1 << 30, 64
+    t = torch.float32 if dtype == "f32" else torch.bfloat16
+    z = torch.full((v,), -2.0, dtype=t, device="cuda")
+    at = [v - 1, 0, v // 2, v // 2 - 1, 12345, v - 12345] + [(i * v) // 59 + 7 for i in range(58)]
+    for i, a in enumerate(at):
+        z[a] = 18.0 - i / 8
+    lse = torch.zeros(1, device="cuda")
+    top, idx = torch.zeros(k, device="cuda"), torch.zeros(k, dtype=torch.int32, device="cuda")
+    rnet.call("rnet_topk_logits_forward", z.data_ptr(), int(dtype == "bf16"), v, 1.0,
+              top.data_ptr(), idx.data_ptr(), lse.data_ptr(), 1, v, k, None)
+    s, out = torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda")
+    tok, par = (torch.full((1,), 9, dtype=torch.int32, device="cuda") for _ in range(2))
+    rnet.call("rnet_beam_select", z.data_ptr(), int(dtype == "bf16"), v, s.data_ptr(), None, -1,
+              out.data_ptr(), tok.data_ptr(), par.data_ptr(), None, 1, 1, v, None)
+    assert rnet.device_error(clear=True) == 0
+    assert idx.tolist() == at and top.tolist() == [18.0 - i / 8 for i in range(64)]
+    want = math.log(sum(math.exp(18.0 - i / 8) for i in range(64)) + (v - 64) * math.exp(-2.0))
+    assert abs(float(lse) - want) <= (2 * 65536 + 200) * U
+    assert tok.tolist() == [v - 1] and par.tolist() == [0]
+    assert abs(float(out) - (18.0 - want)) <= (2 * 65536 + 200) * U
