@@ -64,10 +64,12 @@ struct Standing {
   }
 };
 
-// The W best of the W * S lists, by a whole CTA. W candidates reach the W-th largest
-// of the lists' first ones (of their distinct upper halves); what reaches it is mostly little more than the W, and is
-// ranked by counting (32 x 8 x 256: 3.4 us, 4.2 with a warp that takes the best head W
-// times over).
+// The W best of the W * S lists, by a whole CTA. W candidates reach the W-th largest of
+// the lists' first ones (of their distinct upper halves), and what reaches it is ranked
+// by counting (32 x 8 x 256: 4.2 us, 5.3 with a warp that takes the best head W times
+// over). With many lists, all of them whole rows, that bound is the worst list's and lets
+// most of the W * W through: d * r >= W candidates also reach the r-th largest of the
+// lists' d-th ones, and a warp for each d = 2, 4, .. finds one more bound.
 __device__ __forceinline__ void merge(Lists& in, const SelectArgs& a, size_t m0, int S,
                                       const Standing& now) {
   const int tid = threadIdx.x, W = a.W, lists = W * S;
@@ -114,6 +116,22 @@ __device__ __forceinline__ void merge(Lists& in, const SelectArgs& a, size_t m0,
     if (tid == 0) in.done = done, in.bound = bound, in.totals = 0;
   }
   __syncthreads();
+  if (W > 8 && S == 1) {
+    const int lane = tid & 31, d = 2 << (tid >> 5);
+    if (d <= W) {
+      uint32_t high = 0;
+      if (lane < W && in.n[lane] >= d)
+        high = order((in.score[lane] + (double)key_value(in.key[lane][d - 1])) - in.lse[lane]) >>
+               32;
+      uint32_t bound = __reduce_max_sync(~0u, high);
+      for (int j = d; j < W; j += d) {
+        high = high == bound ? 0 : high;
+        bound = __reduce_max_sync(~0u, high);
+      }
+      if (lane == 0) atomicMax(&in.bound, bound);
+    }
+    __syncthreads();
+  }
   for (int c = tid; c < lists * W; c += blockDim.x) {
     const int list = c / W, i = c % W;
     if (i >= in.n[list]) continue;
