@@ -623,7 +623,9 @@ cudaError_t beam_backtrack(const int* tokens, const int* parents, const float* s
   const int per_warp = 32 / P;
   int warps = (steps + BACK * per_warp - 1) / (BACK * per_warp);
   int ctas = 1;
-  while (ctas < BACK_CTAS && warps > 8 * ctas && (long long)batch * 2 * ctas <= rnet_gemm::num_sms()) ctas *= 2;
+  while (ctas < BACK_CTAS && warps > 8 * ctas &&
+         (long long)batch * 2 * ctas <= rnet_gemm::num_sms())
+    ctas *= 2;
   warps = (warps + ctas - 1) / ctas;
   if (warps > BACK_WARPS) warps = BACK_WARPS;
   const int segments = ctas * warps * per_warp;

@@ -32,8 +32,9 @@ __device__ __forceinline__ void write_place(const TopkArgs& a, size_t row, int k
 
 constexpr int TOPK_WARPS = 4;
 
-// Rows of up to 32 * R words: a warp per row. 64 values a lane spill a little and
-// are still the faster way (4096 rows of 2000 fp32: 18.4 us, 29.9 with a CTA a row).
+// Rows of up to 32 * R words: a warp per row. 64 values a lane take up to 255 registers
+// and are still the faster way (4096 rows of 2000 fp32, top 16: 18 us, 29.5 with a CTA a
+// row; bf16, top 64: 33 and 38).
 template <class T, int R>
 __global__ void __launch_bounds__(32 * TOPK_WARPS) topk_warp_kernel(const T* __restrict__ logits,
                                                                     long long ld, TopkArgs a,
@@ -306,8 +307,8 @@ __device__ __forceinline__ RowGrad row_factors(float P, bool label, const Distil
 // A thread's share of a row: E elements in pieces, and one edge element. The
 // exponentials are kept (KEEP) and only need a factor later. With labels there are
 // two of each: a CTA per row computes them again instead, which leaves room for more
-// CTAs (4096 rows of 8000 fp32: 44.7 us, 57.8 with both kept); a warp per row keeps
-// them (16384 rows of 1000: 32.0 us, 38.4 computed again).
+// CTAs (4096 rows of 8000 fp32: 45 us, 58 with both kept); a warp per row keeps them
+// (16384 rows of 1000: 35.6 us, 39.5 computed again).
 template <class T, int E, bool HARD, bool KEEP>
 struct Share {
   static constexpr int N = Piece<T>::N, NP = E / N;
@@ -399,7 +400,9 @@ __device__ __forceinline__ void zero_pieces(T* d, const Grid<T>& grid, int q0, i
 constexpr int WARPS = 8;  // rows of a CTA of the warp-per-row kernel
 
 // Rows of up to G * E elements in pieces: G lanes per row. With 16 lanes a warp
-// has two rows and what a row costs beside its elements is paid once for both.
+// has two rows and what a row costs beside its elements is paid once for both. Six CTAs
+// to an SM make 8 elements with labels spill 44 to 140 bytes; four, which need no spill,
+// are neither slower nor faster (16384 rows of 256, top 32: 16.5 us, 16.9 with four).
 template <class T, int E, int G, int J, bool HARD>
 __global__ void __launch_bounds__(32 * WARPS, E <= 8 ? 6 : E <= 16 ? 3 : 2) distill_warp_kernel(
     const T* logits, long long ld, T* dlogits, long long ldd, DistillArgs a, int rows) {
@@ -475,8 +478,9 @@ __device__ __forceinline__ void join_parts(const float4* part, int n, float c, f
 }
 
 // Rows of up to 256 * E elements in pieces: a CTA per row, the row in
-// registers. Warp 0 holds the record. As many CTAs to an SM as need no spills (4096
-// rows of 8000 fp32 with labels: 44.6 us with four, 49.6 with three).
+// registers. Warp 0 holds the record. As many CTAs to an SM as need no spills, but for 8
+// bytes of 8 fp32 elements with labels and a long record (4096 rows of 8000 fp32 with
+// labels: 45 us with four, 49.6 with three).
 template <class T, int E, int J, bool HARD>
 constexpr int CTAS = E <= 8 ? 6 : E <= 16 ? 5 : (sizeof(T) == 2 && HARD ? 6 : 5) - J;
 template <class T, int E, int J, bool HARD>
@@ -525,7 +529,8 @@ __global__ void __launch_bounds__(256, CTAS<T, E, J, HARD>)
   }
   if (!d) return;
   const RowGrad g = row_factors(s_P, s_label, a, w, m, s, s1);
-  h.write(d, grid, x, xe, tid, 256, grid.pieces, edge, g, HARD ? 0.f : g.a * rebase(h.m, m, c, a.limit), 0.f);
+  h.write(d, grid, x, xe, tid, 256, grid.pieces, edge, g,
+          HARD ? 0.f : g.a * rebase(h.m, m, c, a.limit), 0.f);
   __syncthreads();  // orders the stores above before those below
   if (warp == 0) r.template fix<HARD>(d, g, a.K, [](int) { return true; });
 }
@@ -748,12 +753,16 @@ template <class T, int J, bool HARD>
 cudaError_t distill_launch(const T* z, long long ld, T* d, long long ldd, const DistillArgs& a,
                            int rows, cudaStream_t s) {
   const int V = a.V;  // at least the elements in pieces
-  if (J == 1 && V <= 32 * 8 && a.K <= 16 && rows >= 2048)
-    // two rows a warp (16384 rows of 256, top 16: 11.4 us, 13.1 with a row each; with
-    // labels 14.2 and 14.9; 1024 rows 4.8 and 4.5). A longer record would take two
+  if constexpr (J == 1) {
+    // two rows a warp (16384 rows of 256, top 16: 10.7 us, 13.3 with a row each; with
+    // labels 13.4 and 15.9; 1024 rows 4.8 and 4.5). A longer record would take two
     // entries a lane, and the search for repeated indices more than it saves.
-    distill_warp<T, 16, 16, J, HARD>(z, ld, d, ldd, a, rows, s);
-  else if (V <= 32 * 8)
+    if (V <= 32 * 8 && a.K <= 16 && rows >= 2048) {
+      distill_warp<T, 16, 16, J, HARD>(z, ld, d, ldd, a, rows, s);
+      return cudaGetLastError();
+    }
+  }
+  if (V <= 32 * 8)
     distill_warp<T, 8, 32, J, HARD>(z, ld, d, ldd, a, rows, s);
   else if (V <= 32 * 16)
     distill_warp<T, 16, 32, J, HARD>(z, ld, d, ldd, a, rows, s);

@@ -1,9 +1,9 @@
-// CPython entries for the operators that a loop calls once a step and whose
-// kernels are shorter than a call through ctypes (2.4 us for the 14 arguments of
-// rnet_beam_select, 0.16 us here). Each is derived from the C function's own type:
-// pointers from int or None, integers from int, floats from float or int. With any
-// other argument, or another number of them, an entry returns NotImplemented and
-// calls nothing.
+// CPython entries for the operators on logits and beams, whose kernels can be shorter
+// than a call through ctypes (2.4 us for the 14 arguments of rnet_beam_select, 0.16 us
+// here). The other functions go through ctypes; a line in `entries` adds one. Each is
+// derived from the C function's own type: pointers from int or None, integers from int,
+// floats from float or int. With any other argument, or another number of them, an
+// entry returns NotImplemented and calls nothing.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
