@@ -1062,7 +1062,8 @@ int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
     d->exec = nullptr;
     d->graph = nullptr;
   }
-  if (use_graph && !d->exec) {
+  // a profiled step is launched kernel by kernel: its events cannot be captured
+  if (use_graph && !d->exec && !prof_on_) {
     // one eager step first so every kernel attribute / tensor map is set up,
     // then capture the step (all arguments are fixed device pointers; the
     // position lives in device memory and is advanced by the argmax kernel)
@@ -1085,7 +1086,7 @@ int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
     d->graph_precision = precision;
   }
   for (int i = 0; i < n_steps; ++i) {
-    if (d->exec) {
+    if (d->exec && !prof_on_) {
       CK(cudaGraphLaunch(d->exec, s));
       rnet_status::count_launch((unsigned)d->graph_kernels);
       d->current = true;
@@ -1158,6 +1159,7 @@ int Engine::beam_search(Decoder* d, int beams, int n_steps, int eos, float alpha
   Decoder::Beam& b = d->beam;
   const int groups = d->M / beams;
   cudaStream_t s = stream_;
+  if (prof_on_) use_graph = false;  // events of a profile cannot be captured
   if (b.exec && (b.beams != beams || b.eos != eos || b.precision != precision)) {
     cudaGraphExecDestroy(b.exec);
     b.exec = nullptr;
