@@ -249,13 +249,13 @@ int rnet_beam_reorder(const void* src, void* dst, size_t row_bytes, size_t row_p
 /* The sequences behind the last beams. tokens / parents [n_steps, batch *
  * beams] are the recorded outputs of n_steps (1..2^30) selections, scores [batch *
  * beams] the last one's. sequences [batch * beams, n_steps]: per sequence the
- * beams sorted by score / length^length_alpha (64 bits, ties to the lower
- * beam; any finite length_alpha, and a score of 0 or -inf stays as it is; NaN counts
- * as -inf, +inf as the largest finite fp32); length counts the tokens up to and
- * including the first eos (n_steps without one, or with eos < 0), and eos fills
- * what follows. lengths and ranked_scores [batch * beams] are in the same order (ranked_scores may be
- * scores). A parent outside 0..beams-1 counts as the beam itself and sets the
- * device error word (bit 1). */
+ * beams sorted by score / length^length_alpha (in 64 bits, from the fp32 numbers
+ * given; ties to the lower beam; any finite length_alpha, and a score of 0 or -inf
+ * stays as it is; NaN counts as -inf, +inf as the largest finite fp32); length
+ * counts the tokens up to and including the first eos (n_steps without one, or with
+ * eos < 0), and eos fills what follows. lengths and ranked_scores [batch * beams]
+ * are in the same order (ranked_scores may be scores). A parent outside
+ * 0..beams-1 counts as the beam itself and sets the device error word (bit 1). */
 int rnet_beam_backtrack(const int* tokens, const int* parents, const float* scores, int eos,
                         float length_alpha, int* sequences, int* lengths, float* ranked_scores,
                         int n_steps, int batch, int beams, void* stream);

@@ -1056,6 +1056,7 @@ int Engine::decode_logits(Decoder* d) {
 
 int Engine::generate(Decoder* d, int n_steps, int* d_out, bool use_graph) {
   cudaStream_t s = stream_;
+  if (n_steps <= 0) return RNET_OK;  // the first capture steps once
   if (d->exec && d->graph_precision != precision) {  // the GEMMs' arithmetic is captured
     cudaGraphExecDestroy(d->exec);
     cudaGraphDestroy(d->graph);
