@@ -781,13 +781,14 @@ cudaError_t distill_launch(const T* z, long long ld, T* d, long long ldd, const 
 
 // Sum of the rows' losses in 64 bits, in a fixed order. Launched so that it may
 // start while the last rows are still at work, and then waits for all of them.
-__global__ void __launch_bounds__(1024) sum_rows_kernel(const float* __restrict__ x, int n,
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const float* __restrict__ x,
+                                                        unsigned n,
                                                         float* __restrict__ out) {
   __shared__ double sh[32];
   rnet_dev::pdl_wait();
   rnet_dev::pdl_trigger();
   double a = 0.0;
-  long long i = threadIdx.x;  // steps past the last of up to 2^31 - 1 rows
+  unsigned i = threadIdx.x;  // steps past the last of up to 2^31 - 1 rows
   for (; i + 7 * 1024 < n; i += 8 * 1024) {
     float v[8];
 #pragma unroll
