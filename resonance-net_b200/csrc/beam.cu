@@ -28,6 +28,8 @@ struct SelectArgs {
   unsigned* err;
 };
 
+constexpr int SELECT_CTAS = 16;  // of one sequence's cluster, where the device places them
+
 // A list per (beam, slice), in that order, largest first.
 struct Lists {
   uint64_t key[RNET_BEAMS_MAX][RNET_BEAMS_MAX];
@@ -63,6 +65,11 @@ struct Standing {
     done = a.finished_in && a.finished_in[m0 + lane / S];
   }
 };
+
+// Candidates that are ranked by counting. Beyond, a warp takes the best head W times over
+// (8 x 32 x 256 of equal logits: 18 us, 129 by counting).
+constexpr int MERGE_COUNT = 128;
+static_assert(SELECT_CTAS * (SELECT_CTAS / 2) <= MERGE_COUNT, "more only from whole rows");
 
 // The W best of the W * S lists, by a whole CTA. W candidates reach the W-th largest of
 // the lists' first ones (of their distinct upper halves), and what reaches it is ranked
@@ -152,31 +159,63 @@ __device__ __forceinline__ void merge(Lists& in, const SelectArgs& a, size_t m0,
     a.tokens[m0 + j] = token;
     if (a.finished) a.finished[m0 + j] = done || token == a.eos;
   };
-  for (int c = tid; c < n; c += blockDim.x) {
-    const uint64_t own = in.total[c];
-    const int which = in.which[c];
-    int place = 0, equal = 0;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const uint64_t t = in.total[k];
-      place += t > own;
-      equal += t == own;
-    }
+  auto choose = [&](int place, int which, uint64_t total) {
     const int list = which >> 5;
-    if (equal > 1) {
-      // the lower beam, then the larger logit or lower token: a row's slices do not show
-      const uint64_t key = in.key[list][which & 31];
+    const bool done = in.done >> list & 1;
+    put(place, (float)unorder(total), list / S,
+        done ? end : key_index(in.key[list][which & 31]), done);
+  };
+  // Equal totals go to the lower beam, then the larger logit or lower token: a row's
+  // slices do not show.
+  if (n <= MERGE_COUNT) {
+    for (int c = tid; c < n; c += blockDim.x) {
+      const uint64_t own = in.total[c];
+      const int which = in.which[c], list = which >> 5;
+      int place = 0, equal = 0;
+#pragma unroll 4
       for (int k = 0; k < n; ++k) {
-        const int other = in.which[k] >> 5, beam = other / S;
-        place += in.total[k] == own &&
-                 (beam < list / S ||
-                  (beam == list / S && in.key[other][in.which[k] & 31] > key));
+        const uint64_t t = in.total[k];
+        place += t > own;
+        equal += t == own;
+      }
+      if (equal > 1 && S == 1) {
+        for (int k = 0; k < n; ++k) place += in.total[k] == own && in.which[k] < which;
+      } else if (equal > 1) {
+        const uint64_t key = in.key[list][which & 31];
+        const int first = list - list % S;  // of the beam's lists
+        for (int k = 0; k < n; ++k) {
+          const int other = in.which[k] >> 5;
+          place += in.total[k] == own &&
+                   (other < first ||
+                    (other < first + S && in.key[other][in.which[k] & 31] > key));
+        }
+      }
+      if (place < W) choose(place, which, own);
+    }
+  } else if (tid < 32) {
+    // ties let many through (of more than 8 beams, so S is 1): a lane to a list, and the
+    // best head W times over, the lowest lane's of equal ones
+    int at = 0;
+    auto next = [&]() -> uint64_t {
+      if (tid >= W || at >= in.n[tid]) return 0;
+      double t = in.score[tid];
+      if (!(in.done >> tid & 1)) t = (t + (double)key_value(in.key[tid][at])) - in.lse[tid];
+      const uint64_t o = order(t);
+      return o > none ? o : 0;
+    };
+    uint64_t head = next();
+    for (int j = 0; j < W; ++j) {
+      const uint32_t high = __reduce_max_sync(~0u, (uint32_t)(head >> 32));
+      const uint32_t low =
+          __reduce_max_sync(~0u, (uint32_t)(head >> 32) == high ? (uint32_t)head : 0u);
+      const uint64_t best = (uint64_t)high << 32 | low;
+      const int from = __ffs(__ballot_sync(~0u, head == best)) - 1;
+      if (tid == from) {
+        choose(j, tid * 32 + at, head);
+        ++at;
+        head = next();
       }
     }
-    if (place >= W) continue;
-    const bool done = in.done >> list & 1;
-    put(place, (float)unorder(own), list / S, done ? end : key_index(in.key[list][which & 31]),
-        done);
   }
   // beams that no candidate is left for
   for (int j = n + tid; j < W; j += blockDim.x) put(j, -INFINITY, j, end, in.done >> (j * S) & 1);
@@ -241,8 +280,6 @@ __global__ void __launch_bounds__(32 * ROWS) beam_select_warps_kernel(
   else __syncthreads();
   if (blockIdx.y == 0) merge(lists, a, m0, 1, now);
 }
-
-constexpr int SELECT_CTAS = 16;  // of one sequence's cluster, where the device places them
 
 // Two CTAs of 512 threads to an SM hide each other's latency better than more
 // values to a thread (32 x 8 rows of 50001 fp32 in L2: 21.1 us with 256 threads of

@@ -48,3 +48,32 @@ def test_deep_lists(rnet, cuda, v, beams, owners):
             # which of two totals that are equal but for rounding comes first is not held
             assert np.all(np.abs(got - best) <= 1e-6), (g, got, best)
             assert len({(a, b) for a, b in zip(p, k)}) == beams
+
+
+@pytest.mark.parametrize("v", [40, 700, 2000, 6001])
+@pytest.mark.parametrize("beams", [12, 17, 32])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_every_candidate_ties(rnet, cuda, v, beams, dtype):
+    """Equal logits everywhere: more candidates than are ranked by counting. Some beams have
+    ended, some have no score, some rows allow fewer tokens than there are beams."""
+    torch, batch = cuda, 4
+    m = batch * beams
+    z = np.zeros((m, v), np.float32)
+    scores, fin = np.full(m, -2.0, np.float32), np.zeros(m, np.int32)
+    fin[beams + 1::5] = 1
+    scores[2 * beams:3 * beams:2] = -np.inf
+    z[3 * beams::3, 5:] = -np.inf
+    t = torch.float32 if dtype == "f32" else torch.bfloat16
+    zz, s, f = (torch.from_numpy(a).cuda() for a in (z, scores, fin))
+    zz = zz.to(t)
+    out = torch.full((m,), 3.0, device="cuda")
+    tok, par, done = (torch.full((m,), 55, dtype=torch.int32, device="cuda") for _ in range(3))
+    rnet.call("rnet_beam_select", zz.data_ptr(), int(dtype == "bf16"), v, s.data_ptr(),
+              f.data_ptr(), 3, out.data_ptr(), tok.data_ptr(), par.data_ptr(), done.data_ptr(),
+              batch, beams, v, None)
+    torch.cuda.synchronize()
+    want = ref.select(z, scores, beams, 3, fin)
+    assert want[4] > 1e-3
+    np.testing.assert_array_equal(tok.cpu().numpy(), want[1])
+    np.testing.assert_array_equal(par.cpu().numpy(), want[2])
+    np.testing.assert_array_equal(done.cpu().numpy(), want[3])
